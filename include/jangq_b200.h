@@ -483,6 +483,65 @@ int jq_ep_combine_residual_rmsnorm(const void* x, const void* y, int k, int64_t 
                                    int act_dtype, const uint64_t* peer_bufs, int rank, int world, int64_t tcap,
                                    int32_t* counters, int emulate_ranks, jq_stream_t stream);
 
+/* score kinds of jq_moe_route_topk */
+#define JQ_SCORE_SOFTMAX 0
+#define JQ_SCORE_SIGMOID 1
+
+/* Router selection with a choice of scores, a balance bias and groups of experts, over logits from a GEMM.  Per row:
+ *   s = softmax(l) or 1 / (1 + exp(-l)),   c = s + bias (bias: num_experts float32, or NULL)
+ *   groups > 1: experts [g E/groups, (g+1) E/groups) form group g, whose score is the sum of its group_top (1 or 2)
+ *   largest c; experts outside the groups_kept best groups (ties: the lower group) are not chosen
+ *   idx = the k largest c, descending, ties to the lower expert;   w = s[idx], / (their sum + 1e-20) when renorm, * scale
+ * c is compared in float64, so the choice is the one of the exact scores up to 1e-16.  A NaN logit counts as -inf (score
+ * zero); k may not exceed the experts of the kept groups.  With softmax, no bias and one group it is jq_moe_topk's
+ * selection.  logits [T, ld >= num_experts] f32, f16 or bf16; idx_out int32 [T, k], w_out f32 [T, k]; num_experts <= 1024,
+ * groups <= 32.  The reference's routers: dots3/ops.py:149-162 and dsv41/model.py:1171-1191. */
+int jq_moe_route_topk(const void* logits, int logits_dtype, int64_t ld, int64_t T, int num_experts, int k, int score,
+                      const float* bias, int groups, int groups_kept, int group_top, int renorm, float scale,
+                      int32_t* idx_out, float* w_out, jq_stream_t stream);
+
+/* MXFP4 (OCP microscaling): blocks of 32 along K share a power of two 2^(byte - 127), a code is e2m1 (sign, two exponent
+ * bits, one mantissa bit: 0 .5 1 1.5 2 3 4 6).  codes uint32 [rows, K/8], the first of a word's eight codes in its lowest
+ * bits (the affine codec's 4-bit layout); scales uint8 [rows, K/32]; K % 32 == 0.
+ *
+ * jq_mxfp4_quantize: byte - 127 = floor(log2(max |w|)) - 2 of the block (not below -127), codes to the nearest, ties to the
+ *   even code, 6 and above to 6; a block with an infinity or a NaN gets byte 255 (not a number).  w contiguous, 16-byte
+ *   aligned, f32, f16 or bf16.
+ * jq_mxfp4_dequantize: the values, rounded once to out_dtype (exact in bf16 and f32 but for overflow). */
+int jq_mxfp4_quantize(const void* w, int w_dtype, int64_t rows, int64_t K, uint32_t* codes, uint8_t* scales,
+                      jq_stream_t stream);
+int jq_mxfp4_dequantize(const uint32_t* codes, const uint8_t* scales, int64_t rows, int64_t K, void* out, int out_dtype,
+                        jq_stream_t stream);
+
+/* y[M, N] = x[M, K] . deq(w)[N, K]^T, x and y of one 16-bit type, f32 sums.  The weight enters in x's type: exact in bf16,
+ * rounded once in f16 (scales below 2^-23, and overflow to infinity above 2^13).  x 16-byte aligned with ldx % 8 == 0,
+ * codes 16-byte, scales 2-byte aligned.
+ *   jq_mxfp4_gemv: M <= 16, any K % 32 == 0;   jq_mxfp4_gemm: any M, K % 64 == 0 (tensor cores).
+ * jq_mxfp4_gather_gemv: y[p] = x[p / x_div] . deq(w[pair_expert[p] - expert_base])^T for the pairs of routed experts; codes
+ *   [num_experts, N, K/8] and scales [num_experts, N, K/32] are stacked; pairs of other experts get rows of zeros.
+ * jq_mxfp4_moe_gemm, jq_mxfp4_moe_gate_up_swiglu: jq_moe_gemm_tiled and jq_moe_gate_up_swiglu over MXFP4 experts (tile
+ *   lists of 128 or 192 rows, pointer tables to codes and scales, which must be 16- and 2-byte aligned).
+ * jq_mxfp4_gemm4: both operands in MXFP4 on the block-scaled tensor-core path, y f32, f16 or bf16; any M, K % 32 == 0. */
+int jq_mxfp4_gemv(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint32_t* codes, const uint8_t* scales,
+                  int64_t N, int64_t K, void* y, int64_t ldy, jq_stream_t stream);
+int jq_mxfp4_gemm(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint32_t* codes, const uint8_t* scales,
+                  int64_t N, int64_t K, void* y, int64_t ldy, jq_stream_t stream);
+int jq_mxfp4_gather_gemv(const void* x, int x_dtype, int64_t ldx, int x_div, const int32_t* pair_expert, int64_t P,
+                         const uint32_t* codes, const uint8_t* scales, int num_experts, int expert_base, int64_t N,
+                         int64_t K, void* y, int64_t ldy, jq_stream_t stream);
+int jq_mxfp4_moe_gemm(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx, const int32_t* expert_offsets,
+                      const int32_t* tile_expert, const int32_t* tile_row0, const int32_t* num_tiles, int64_t max_tiles,
+                      int tile_m, const uint32_t* const* codes_tab, const uint8_t* const* scales_tab, int64_t N, int64_t K,
+                      void* y_sorted, int64_t ldy, jq_stream_t stream);
+int jq_mxfp4_moe_gate_up_swiglu(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx,
+                                const int32_t* expert_offsets, const int32_t* tile_expert, const int32_t* tile_row0,
+                                const int32_t* num_tiles, int64_t max_tiles, int tile_m, const uint32_t* const* gate_codes,
+                                const uint8_t* const* gate_scales, const uint32_t* const* up_codes,
+                                const uint8_t* const* up_scales, int64_t N, int64_t K, const float* weights,
+                                const int32_t* order, float limit, void* h, int64_t ldh, jq_stream_t stream);
+int jq_mxfp4_gemm4(const uint32_t* xcodes, const uint8_t* xscales, int64_t M, const uint32_t* wcodes,
+                   const uint8_t* wscales, int64_t N, int64_t K, void* y, int y_dtype, int64_t ldy, jq_stream_t stream);
+
 /* Reads the device-side status word (synchronises the device).  JQ_ETIMEOUT when a
  * kernel's bounded wait on a copy in flight ran out since the library was loaded.
  * No counterpart in the reference: its Metal path has no device-side waits. */

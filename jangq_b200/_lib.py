@@ -22,6 +22,7 @@ JQ_QUANT_MSE_EXHAUSTIVE = 2
 JQ_QUANT_IEEE_DIV = 4
 JQ_GEMV_STATIC_WEIGHTS = 1
 JQ_GATHER_FEW_LOCAL = 2
+JQ_SCORE_SOFTMAX, JQ_SCORE_SIGMOID = 0, 1
 QGEMV_MAX_M = 16
 QGEMV_MAX_BATCH = 8
 MOE_TILE_M = 128
@@ -109,6 +110,16 @@ SIGNATURES = {
     "jq_ep_buffer_bytes": (C.c_size_t, [_i64, _i64]),
     "jq_ep_combine_residual_rmsnorm": (C.c_int, [_p, _p, _i32, _i64, _i64, C.c_float, _p, _i32, _p, _i32, _i32, _i64,
                                                  _p, _i32, _p]),
+    "jq_moe_route_topk": (C.c_int, [_p, _i32, _i64, _i64, _i32, _i32, _i32, _p, _i32, _i32, _i32, _i32, C.c_float, _p, _p, _p]),
+    "jq_mxfp4_quantize": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _p]),
+    "jq_mxfp4_dequantize": (C.c_int, [_p, _p, _i64, _i64, _p, _i32, _p]),
+    "jq_mxfp4_gemv": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p]),
+    "jq_mxfp4_gemm": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p]),
+    "jq_mxfp4_gather_gemv": (C.c_int, [_p, _i32, _i64, _i32, _p, _i64, _p, _p, _i32, _i32, _i64, _i64, _p, _i64, _p]),
+    "jq_mxfp4_moe_gemm": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _p, _p, _i64, _i64, _p, _i64, _p]),
+    "jq_mxfp4_moe_gate_up_swiglu": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _p, _p, _p, _p, _i64, _i64, _p,
+                                              _p, C.c_float, _p, _i64, _p]),
+    "jq_mxfp4_gemm4": (C.c_int, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _i32, _i64, _p]),
     "jq_gather_qgemv": (C.c_int, [_p, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p, _i32, _i32, _i64, _i64, _i32, _i32,
                                   _p, _i64, _p]),
 }

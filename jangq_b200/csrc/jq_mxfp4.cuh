@@ -1,0 +1,74 @@
+// Microscaled 4-bit floating point (OCP MX): 32 numbers share a power of two 2^(byte - 127), a number is e2m1: sign, two
+// exponent bits, one mantissa bit, values 0 .5 1 1.5 2 3 4 6.  Byte 255 marks a block that is not a number.
+#pragma once
+
+#include "jq_mma.cuh"
+#include "jq_ts.cuh"
+
+namespace jq {
+
+constexpr int MX_BLOCK = 32;
+
+int check_mxfp4_shape(int64_t rows, int64_t K);
+
+// ---- expansion to a 16-bit float type -----------------------------------------------------------------
+// The three low bits of a code placed at the top of the type's mantissa and the bottom of its exponent read as the code's
+// value times 2^-126 (bf16) or 2^-14 (f16), zero and the subnormal 0.5 included, so the scale goes in with the multiply
+// that lifts them: one product per two weights, and nothing is rounded where the type holds the weight.
+template <typename AT> struct Mx;
+template <> struct Mx<__nv_bfloat16> {
+    static constexpr int POS = 6;                        // bit of the code's mantissa bit
+    static constexpr uint32_t MASK = 0x01C001C0u;
+    static constexpr int FAST_MAX = 128;                 // largest byte whose lift is a bf16 number
+    // 2^(byte - 1), twice
+    __device__ static __forceinline__ uint32_t lift(uint32_t b) { return ((b + 126u) << 7) * 0x00010001u; }
+    // the product for any byte: up to 2^127, then the rest
+    __device__ static __forceinline__ uint32_t any(uint32_t field, uint32_t b) {
+        if (b <= FAST_MAX) return P2<__nv_bfloat16>::fma(field, lift(b), 0x80008000u);
+        const uint32_t rest = b == 255u ? 0x7FC0u : (b - 1u) << 7;                       // 2^(b - 128)
+        return P2<__nv_bfloat16>::fma(P2<__nv_bfloat16>::fma(field, lift(128u), 0x80008000u), rest * 0x00010001u, 0x80008000u);
+    }
+};
+template <> struct Mx<__half> {
+    static constexpr int POS = 9;
+    static constexpr uint32_t MASK = 0x0E000E00u;
+    static constexpr int FAST_MAX = 128;
+    // 2^(byte - 113), twice; zero below 2^-24, where no weight of the block reaches half of f16's smallest number
+    __device__ static __forceinline__ uint32_t lift(uint32_t b) {
+        const uint32_t h = b >= 99u ? (b - 98u) << 10 : (b >= 89u ? 1u << (b - 89u) : 0u);
+        return h * 0x00010001u;
+    }
+    __device__ static __forceinline__ uint32_t any(uint32_t field, uint32_t b) {
+        if (b <= FAST_MAX) return P2<__half>::fma(field, lift(b), 0x80008000u);
+        const uint32_t one = P2<__half>::fma(field, lift(128u), 0x80008000u);             // twice the code's value
+        const uint32_t e1 = min(b - 128u, 15u), e2 = min(b - 128u - e1, 15u);             // 2^30 overflows every weight
+        const uint32_t m1 = b == 255u ? 0x7E00u : (e1 + 15u) << 10, m2 = (e2 + 15u) << 10;
+        return P2<__half>::fma(P2<__half>::fma(one, m1 * 0x00010001u, 0x80008000u), m2 * 0x00010001u, 0x80008000u);
+    }
+};
+
+// code fields (j, j + 4) of a word of eight codes, j = 0 .. 3: sign at bit 15, the rest at POS
+template <typename AT, int J>
+__device__ __forceinline__ uint32_t mx_field(uint32_t w) {
+    constexpr int up = 12 - 4 * J, at = Mx<AT>::POS - 4 * J;
+    const uint32_t s = up > 0 ? w << up : w;
+    const uint32_t m = at >= 0 ? w << at : w >> -at;
+    return (s & 0x80008000u) | (m & Mx<AT>::MASK);
+}
+// eight codes -> pairs (0,4) (1,5) (2,6) (3,7), scaled
+template <typename AT>
+__device__ __forceinline__ void mx_expand8(uint32_t w, uint32_t lift, uint32_t (&o)[4]) {
+    o[0] = P2<AT>::fma(mx_field<AT, 0>(w), lift, 0x80008000u);
+    o[1] = P2<AT>::fma(mx_field<AT, 1>(w), lift, 0x80008000u);
+    o[2] = P2<AT>::fma(mx_field<AT, 2>(w), lift, 0x80008000u);
+    o[3] = P2<AT>::fma(mx_field<AT, 3>(w), lift, 0x80008000u);
+}
+template <typename AT>
+__device__ __forceinline__ void mx_expand8_any(uint32_t w, uint32_t byte, uint32_t (&o)[4]) {
+    o[0] = Mx<AT>::any(mx_field<AT, 0>(w), byte);
+    o[1] = Mx<AT>::any(mx_field<AT, 1>(w), byte);
+    o[2] = Mx<AT>::any(mx_field<AT, 2>(w), byte);
+    o[3] = Mx<AT>::any(mx_field<AT, 3>(w), byte);
+}
+
+}  // namespace jq

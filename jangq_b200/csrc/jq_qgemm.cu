@@ -34,6 +34,7 @@
 #include <atomic>
 #include <mutex>
 
+#include "jq_mxfp4.cuh"
 #include "jq_ts.cuh"
 
 namespace jq {
@@ -144,6 +145,38 @@ __device__ __forceinline__ void expand_block(const uint8_t* crow, int r, int kbi
     }
 }
 
+// The same for MXFP4 rows: 4-bit codes at the same places, and per k-block two scale bytes that travel as one 16-bit
+// sidecar with group size 64 (no bias).  Exact in bf16; in f16 one rounding (jq_mxfp4.cuh).
+template <typename AT>
+__device__ __forceinline__ void expand_block_mx(const uint8_t* crow, int r, int kbi, int kb, int kb_next, const uint16_t* side,
+                                                Sidecars& sc, uint32_t (&out)[32]) {
+    constexpr int CPR = CodeStage<4>::RB / 16;
+    const uint4* cp = reinterpret_cast<const uint4*>(crow);
+    uint32_t sb;
+    if (sc.mode != 0) {
+        sb = side[kb & 3];
+    } else {
+        sb = sc.ns;
+        if (kb_next >= 0) sc.fetch(kb_next);
+    }
+    const bool fast = __all_sync(0xFFFFFFFFu, max(sb & 255u, sb >> 8) <= (uint32_t)Mx<AT>::FAST_MAX);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint4 v = cp[code_chunk<CPR>(kbi * 2 + h, r)];
+        const uint32_t cur[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t byte = h ? sb >> 8 : sb & 255u, lift = Mx<AT>::lift(byte);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t f[4];                                   // codes (j, j + 4)
+            if (fast) mx_expand8<AT>(cur[i], lift, f);
+            else mx_expand8_any<AT>(cur[i], byte, f);
+            uint32_t* o = out + 16 * h + 4 * i;
+            o[0] = prmt(f[0], f[1], 0x5410); o[1] = prmt(f[2], f[3], 0x5410);
+            o[2] = prmt(f[0], f[1], 0x7632); o[3] = prmt(f[2], f[3], 0x7632);
+        }
+    }
+}
+
 // 32 accumulator columns (activation rows row0 .. row0 + 31 of y, `rows` of them valid) of one weight row per lane
 template <typename AT>
 __device__ __forceinline__ void store_columns(const GemmArgs& a, const uint32_t (&v)[32], int64_t row0, int rows, int64_t nn,
@@ -209,7 +242,8 @@ template <int BITS> struct GemmCfg {
 // accumulates its share of the k-blocks in its own tensor memory and leaves the sums as float32 in its (by then
 // idle) shared memory; after a cluster barrier CTA r adds and stores the activation rows of its share, in rank order.
 // Both cluster barriers are reached by every thread on every path.
-template <typename AT, int BITS, int KS>
+// MX: MXFP4 rows (BITS 4, group size 64: see expand_block_mx).
+template <typename AT, int BITS, int KS, bool MX = false>
 __global__ void __launch_bounds__(GemmCfg<BITS>::THREADS, 1)
 qgemm_ts_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
     using A = Act<AT>;
@@ -300,7 +334,7 @@ qgemm_ts_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
         int buf = 0, slot = 0;
         uint32_t phase = 1u;
         const SideSrc side = {a.scales, a.biases, nullptr, nullptr, a.G, side_mode(a.scales, a.biases, a.G, a.gs)};
-        ok = load_codes<BITS, CD>(a.codes, n0, a.N, a.K, kb0 / CKB, nst, sC, cfull, cempty, threadIdx.x - 64, buf, phase, side,
+        ok = load_codes<BITS, CD, false, !MX>(a.codes, n0, a.N, a.K, kb0 / CKB, nst, sC, cfull, cempty, threadIdx.x - 64, buf, phase, side,
                                      sSide, slot);
         cp_async_commit();
         cp_async_wait<0>();
@@ -328,8 +362,11 @@ qgemm_ts_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
             if (i < nkb) {
                 const int kb = kb0 + i;                        // absolute k-block
                 uint32_t out[32];
-                expand_block<AT, BITS>(sC + cb * C::C_STAGE + r * RB, r, i % CKB, kb, i + RA < nkb ? kb + RA : -1,
-                                       reinterpret_cast<const uint16_t*>(sSide + slot * SIDE_SLOT) + r * 4, sc, out);
+                const uint8_t* crow = sC + cb * C::C_STAGE + r * RB;
+                const uint16_t* side = reinterpret_cast<const uint16_t*>(sSide + slot * SIDE_SLOT) + r * 4;
+                const int kb_next = i + RA < nkb ? kb + RA : -1;
+                if constexpr (MX) expand_block_mx<AT>(crow, r, i % CKB, kb, kb_next, side, sc, out);
+                else expand_block<AT, BITS>(crow, r, i % CKB, kb, kb_next, side, sc, out);
                 if (++slot == CD) slot = 0;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(cempty + cb);
@@ -467,7 +504,7 @@ template <bool GU> __device__ __forceinline__ int pers_side_mode(const GemmArgs&
     return m == 0 || m2 == 0 ? 0 : max(m, m2);               // the copy that both matrices are aligned for
 }
 
-template <typename AT, int BITS, bool GU, int TN>
+template <typename AT, int BITS, bool GU, int TN, bool MX = false>
 __global__ void __launch_bounds__(PersCfg<BITS, TN>::THREADS, 1)
 qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
     using C = PersCfg<BITS, TN>;
@@ -572,7 +609,7 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
             const PersTile t = take(tile);
             if (t.rows <= 0) continue;
             const SideSrc side = {t.scales, t.biases, t.scales2, t.biases2, a.G, pers_side_mode<GU>(a, t)};
-            ok = load_codes<BITS, CD, GU>(t.codes, t.n0, a.N, a.K, 0, nst, sC, cfull, cempty, threadIdx.x - 64, buf, ph, side,
+            ok = load_codes<BITS, CD, GU, !MX>(t.codes, t.n0, a.N, a.K, 0, nst, sC, cfull, cempty, threadIdx.x - 64, buf, ph, side,
                                              smem + C::SIDE_OFF, slot, t.codes2);
         }
         cp_async_commit();
@@ -664,9 +701,11 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
                 if (buf >= 2 * CD) buf -= 2 * CD;
                 if (kb < nkb) {
                     uint32_t out[32];
-                    expand_block<AT, BITS>(sC + cb * C::C_STAGE + r * RB, r, kb % CKB, kb, kb + RA < nkb ? kb + RA : -1,
-                                           reinterpret_cast<const uint16_t*>(smem + C::SIDE_OFF + slot * SIDE_SLOT) + r * 4, sc,
-                                           out);
+                    const uint8_t* crow = sC + cb * C::C_STAGE + r * RB;
+                    const uint16_t* side = reinterpret_cast<const uint16_t*>(smem + C::SIDE_OFF + slot * SIDE_SLOT) + r * 4;
+                    const int kb_next = kb + RA < nkb ? kb + RA : -1;
+                    if constexpr (MX) expand_block_mx<AT>(crow, r, kb % CKB, kb, kb_next, side, sc, out);
+                    else expand_block<AT, BITS>(crow, r, kb % CKB, kb, kb_next, side, sc, out);
                     if (++slot == CD) slot = 0;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(cempty + cb);
@@ -715,12 +754,12 @@ EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
-template <typename AT, int BITS, int KS>
+template <typename AT, int BITS, int KS, bool MX = false>
 static int launch_gemm(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_tiles, cudaStream_t st) {
     using C = GemmCfg<BITS>;
     constexpr size_t smem = C::SMEM;
     static_assert(smem <= GEMM_SMEM, "shared memory of one CTA");
-    auto kernel = qgemm_ts_kernel<AT, BITS, KS>;
+    auto kernel = qgemm_ts_kernel<AT, BITS, KS, MX>;
     static bool attr_done[64] = {};
     int dev = 0;
     JQ_CUDA_OK(cudaGetDevice(&dev));
@@ -747,11 +786,11 @@ static int launch_gemm(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_til
     return check_launch("qgemm");
 }
 
-template <typename AT, int BITS, bool GU, int TN>
+template <typename AT, int BITS, bool GU, int TN, bool MX = false>
 static int launch_pers(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_tiles, cudaStream_t st) {
     using C = PersCfg<BITS, TN>;
     static_assert(C::SMEM <= GEMM_SMEM, "shared memory of one CTA");
-    auto kernel = qgemm_pers_kernel<AT, BITS, GU, TN>;
+    auto kernel = qgemm_pers_kernel<AT, BITS, GU, TN, MX>;
     static bool attr_done[64] = {};
     int dev = 0;
     JQ_CUDA_OK(cudaGetDevice(&dev));
@@ -783,10 +822,11 @@ struct GroupedArgs {
 };
 
 // Dense when grp == nullptr (codes/scales/biases of one matrix); grouped otherwise (x holds the M
-// expert-sorted rows, the weight pointers come from the tables).
+// expert-sorted rows, the weight pointers come from the tables).  mx: MXFP4 weights; bits 4, gs 64, and the scale bytes as
+// 16-bit sidecars (the biases are not read).
 int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint32_t* codes, const void* scales,
                    const void* biases, int sidecar_dtype, int64_t N, int64_t K, int bits, int gs, void* y,
-                   int y_dtype, int64_t ldy, const GroupedArgs* grp, cudaStream_t st) {
+                   int y_dtype, int64_t ldy, const GroupedArgs* grp, cudaStream_t st, bool mx = false) {
     int rc = check_quant_shape(N, K, bits, gs);
     if (rc != JQ_OK) return rc;
     JQ_REQUIRE(M >= 0, JQ_EINVAL, "negative M");
@@ -884,6 +924,18 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
         if (ks == 2) return launch_gemm<T, B, 2>(xmap, a, m_tiles, st);                                   \
         return launch_gemm<T, B, 1>(xmap, a, m_tiles, st);                                                \
     }
+#define JQ_GEMM_MX(T)                                                                                     \
+    {                                                                                                     \
+        if (gu) return launch_pers<T, 4, true, 192, true>(xmap, a, m_tiles, st);                          \
+        if (grp) return launch_pers<T, 4, false, 192, true>(xmap, a, m_tiles, st);                        \
+        if (ks == 4) return launch_gemm<T, 4, 4, true>(xmap, a, m_tiles, st);                             \
+        if (ks == 2) return launch_gemm<T, 4, 2, true>(xmap, a, m_tiles, st);                             \
+        return launch_gemm<T, 4, 1, true>(xmap, a, m_tiles, st);                                          \
+    }
+    if (mx) {
+        if (x_dtype == JQ_BF16) JQ_GEMM_MX(__nv_bfloat16)
+        JQ_GEMM_MX(__half)
+    }
 #define JQ_GEMM_CASE(B)                                                                                   \
     if (bits == B) {                                                                                      \
         if (grp && grp->tile_m == 256)                         /* bf16 only, see above */                 \
@@ -894,6 +946,7 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
     }
     JQ_GEMM_CASE(2) JQ_GEMM_CASE(3) JQ_GEMM_CASE(4) JQ_GEMM_CASE(5) JQ_GEMM_CASE(6) JQ_GEMM_CASE(8)
 #undef JQ_GEMM_CASE
+#undef JQ_GEMM_MX
 #undef JQ_GEMM_T
     return fail(JQ_EUNSUPPORTED, "bits=%d", bits);
 }
@@ -963,6 +1016,14 @@ static int static_tiles_ptr(int32_t** out) {
         cached[dev].store(p, std::memory_order_release);
     }
     *out = p;
+    return JQ_OK;
+}
+
+// MXFP4 rows of whole 64-code k-blocks
+static int check_mxfp4_gemm(int64_t N, int64_t K) {
+    int rc = check_mxfp4_shape(N, K);
+    if (rc != JQ_OK) return rc;
+    JQ_REQUIRE(K % GEMM_BK == 0, JQ_EUNSUPPORTED, "the tensor-core products need K to be a multiple of 64, got %lld", (long long)K);
     return JQ_OK;
 }
 
@@ -1059,6 +1120,62 @@ int jq_moe_gate_up_swiglu(const void* x_sorted, int act_dtype, int64_t max_rows,
     g.wts = weights; g.order = order; g.lim = limit;
     return qgemm_dispatch(x_sorted, act_dtype, max_rows, ldx, nullptr, nullptr, nullptr, sidecar_dtype, N, K, bits,
                           group_size, h, act_dtype, ldh, &g, (cudaStream_t)stream);
+}
+
+int jq_mxfp4_gemm(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint32_t* codes, const uint8_t* scales, int64_t N,
+                  int64_t K, void* y, int64_t ldy, jq_stream_t stream) {
+    using namespace jq;
+    int rc = check_mxfp4_gemm(N, K);
+    if (rc != JQ_OK) return rc;
+    JQ_REQUIRE(aligned(scales, 2), JQ_EINVAL, "scales must be 2-byte aligned");
+    return qgemm_dispatch(x, x_dtype, M, ldx, codes, scales, scales, x_dtype, N, K, 4, 64, y, x_dtype, ldy, nullptr,
+                          (cudaStream_t)stream, true);
+}
+
+int jq_mxfp4_moe_gemm(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx, const int32_t* expert_offsets,
+                      const int32_t* tile_expert, const int32_t* tile_row0, const int32_t* num_tiles, int64_t max_tiles,
+                      int tile_m, const uint32_t* const* codes_tab, const uint8_t* const* scales_tab, int64_t N, int64_t K,
+                      void* y_sorted, int64_t ldy, jq_stream_t stream) {
+    using namespace jq;
+    int rc = check_mxfp4_gemm(N, K);
+    if (rc != JQ_OK) return rc;
+    JQ_REQUIRE(tile_m == 128 || tile_m == 192, JQ_EINVAL, "tile_m must be 128 or 192");
+    JQ_REQUIRE(expert_offsets && tile_expert && tile_row0 && num_tiles && codes_tab && scales_tab, JQ_EINVAL, "null pointer");
+    JQ_REQUIRE(max_tiles >= 0, JQ_EINVAL, "negative max_tiles");
+    GroupedArgs g;
+    g.tile_expert = tile_expert; g.tile_row0 = tile_row0; g.num_tiles = num_tiles; g.expert_offsets = expert_offsets;
+    g.bits_tab = nullptr; g.codes_tab = codes_tab;
+    g.scales_tab = g.biases_tab = reinterpret_cast<const void* const*>(scales_tab);
+    g.max_tiles = max_tiles;
+    g.tile_m = tile_m;
+    return qgemm_dispatch(x_sorted, act_dtype, max_rows, ldx, nullptr, nullptr, nullptr, act_dtype, N, K, 4, 64, y_sorted,
+                          act_dtype, ldy, &g, (cudaStream_t)stream, true);
+}
+
+int jq_mxfp4_moe_gate_up_swiglu(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx,
+                                const int32_t* expert_offsets, const int32_t* tile_expert, const int32_t* tile_row0,
+                                const int32_t* num_tiles, int64_t max_tiles, int tile_m, const uint32_t* const* gate_codes,
+                                const uint8_t* const* gate_scales, const uint32_t* const* up_codes,
+                                const uint8_t* const* up_scales, int64_t N, int64_t K, const float* weights,
+                                const int32_t* order, float limit, void* h, int64_t ldh, jq_stream_t stream) {
+    using namespace jq;
+    int rc = check_mxfp4_gemm(N, K);
+    if (rc != JQ_OK) return rc;
+    JQ_REQUIRE(tile_m == 128 || tile_m == 192, JQ_EINVAL, "tile_m must be 128 or 192");
+    JQ_REQUIRE(expert_offsets && tile_expert && tile_row0 && num_tiles && gate_codes && gate_scales && up_codes && up_scales,
+               JQ_EINVAL, "null pointer");
+    JQ_REQUIRE(weights == nullptr || order != nullptr, JQ_EINVAL, "routing weights need the sort order");
+    JQ_REQUIRE(max_tiles >= 0, JQ_EINVAL, "negative max_tiles");
+    GroupedArgs g;
+    g.tile_expert = tile_expert; g.tile_row0 = tile_row0; g.num_tiles = num_tiles; g.expert_offsets = expert_offsets;
+    g.bits_tab = nullptr; g.codes_tab = gate_codes; g.codes_tab2 = up_codes;
+    g.scales_tab = g.biases_tab = reinterpret_cast<const void* const*>(gate_scales);
+    g.scales_tab2 = g.biases_tab2 = reinterpret_cast<const void* const*>(up_scales);
+    g.max_tiles = max_tiles;
+    g.tile_m = tile_m;
+    g.wts = weights; g.order = order; g.lim = limit;
+    return qgemm_dispatch(x_sorted, act_dtype, max_rows, ldx, nullptr, nullptr, nullptr, act_dtype, N, K, 4, 64, h, act_dtype,
+                          ldh, &g, (cudaStream_t)stream, true);
 }
 
 }  // extern "C"

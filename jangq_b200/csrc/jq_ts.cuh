@@ -316,7 +316,8 @@ template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, co
 // (0, 1) at the start: the first pass finds every stage empty.  Returns false when a wait ran out; the caller waits for
 // the copies in flight.
 //   codes2 (PAIR): the tile is rows [n0, n0 + 64) of two matrices, the second one's behind the first one's
-template <int BITS, int CD, bool PAIR = false>
+//   BIAS: false for codes whose only sidecar is the scale (the chunk's second half stays unused)
+template <int BITS, int CD, bool PAIR = false, bool BIAS = true>
 __device__ __forceinline__ bool load_codes(const uint32_t* codes, int64_t n0, int64_t N, int64_t K, int st0, int nst,
                                            uint8_t* sC, uint64_t* cfull, uint64_t* cempty, int l, int& buf,
                                            uint32_t& phase, const SideSrc& side, uint8_t* sSide, int& slot,
@@ -365,7 +366,7 @@ __device__ __forceinline__ bool load_codes(const uint32_t* codes, int64_t n0, in
             if (side.mode != 0) {                      // change from tile to tile, and the dequantizers count every chunk
                 const uint32_t sd = smem_u32(sSide) + (uint32_t)(slot * SIDE_SLOT + l * 8);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {                              // scales of both rows, then biases
+                for (int i = 0; i < (BIAS ? 4 : 2); ++i) {                 // scales of both rows, then biases
                     const uint32_t di = sd + (uint32_t)(i * 64 * 8);
                     if (side.mode == 1) {
                         cp_async_small<8>(di, sp[i] + soffb);

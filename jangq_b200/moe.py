@@ -4,6 +4,7 @@
                       optionally with a different bit width per expert
     gather_qmm        <-> mx.gather_qmm call shape of jang_tools/dots3/ops.py:168-192
     route_softmax_topk  softmax -> top-k -> renormalise (dots3/ops.py:159-162 normalisation)
+    route_topk        the same with sigmoid scores, a balance bias for the choice and groups of experts
     moe_layer         the layer logic of dsv41/model.py:1206-1245 (sort by expert above 64 pairs,
                       SwiGLU with optional clamp, routing weight applied before down, f32 sum over
                       slots, optional shared expert)
@@ -19,6 +20,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import JangqError
+from .mxfp4 import MXFP4ExpertBank, expert_gemm, expert_gemv, rows_ok
 
 SORT_THRESHOLD = 64      # pairs; dsv41/model.py:1206 (n * topk >= 64), mlx-lm SwitchGLU indices.size >= 64
 
@@ -272,6 +274,44 @@ def route_softmax_topk(logits: torch.Tensor, k: int, renorm: bool = True, scale:
     return idx.to(torch.int32), (w * scale).float()
 
 
+_SCORES = {"softmax": _lib.JQ_SCORE_SOFTMAX, "sigmoid": _lib.JQ_SCORE_SIGMOID}
+
+
+def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+               groups_kept: int = 1, group_top: int = 2, renorm: bool = True, scale: float = 1.0):
+    """(idx int32 [T, k], w float32 [T, k]) of logits [T, E]: route_softmax_topk with a choice of scores, a balance bias and
+    groups of experts (dots3/ops.py:149-162, dsv41/model.py:1171-1191).
+
+    s = softmax(logits) or sigmoid(logits); experts are chosen by c = s + bias (bias [E], for the choice only).  With
+    groups > 1 the E / groups experts of a group stand together, a group's score is the sum of its `group_top` (1 or 2)
+    largest c, and only experts of the `groups_kept` best groups can be chosen.  idx is in descending order of c, ties to
+    the lower expert (and the lower group); w = s[idx], divided by their sum + 1e-20 with renorm, times scale.  NaN
+    logits count as -inf.  E <= 1024, groups <= 32."""
+    dev = _lib.require_cuda(logits, bias)
+    lib = _lib.load()
+    if logits.dim() != 2:
+        raise JangqError(_lib.JQ_EINVAL, f"logits must be [T, E], got {tuple(logits.shape)}")
+    if score not in _SCORES:
+        raise JangqError(_lib.JQ_EINVAL, f"unknown score {score!r}; use 'softmax' or 'sigmoid'")
+    T, E = logits.shape
+    if bias is not None:
+        if bias.shape != (E,) or not bias.is_floating_point():
+            raise JangqError(_lib.JQ_EINVAL, f"bias must be a float tensor [{E}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.float().contiguous()
+    # the pitch of a single row says nothing, and a broadcast one (0) names no rows
+    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
+        logits = logits.contiguous()
+    # sizes a table cannot have are refused by the library; nothing of theirs is allocated before
+    idx = torch.empty((T, max(k, 0)), dtype=torch.int32, device=dev)
+    w = torch.empty((T, max(k, 0)), dtype=torch.float32, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(lib.jq_moe_route_topk(logits.data_ptr(), _lib.dtype_id(logits.dtype), logits.stride(0) if T > 1 else E, T, E,
+                                         k, _SCORES[score], bias.data_ptr() if bias is not None else None, groups, groups_kept,
+                                         group_top, 1 if renorm else 0, float(scale), idx.data_ptr(), w.data_ptr(),
+                                         _lib.stream_ptr(dev)))
+    return idx, w
+
+
 def route_from_hidden(x: torch.Tensor, router_w: torch.Tensor, k: int, renorm: bool = True, scale: float = 1.0):
     """route_softmax_topk(x @ router_w.T, k) in one launch for few tokens: (idx int32 [T, k], w f32 [T, k]).
     x [T, H] and router_w [E, H] share a 16-bit dtype; E <= 1024."""
@@ -376,6 +416,52 @@ def _shared_expert(x: torch.Tensor, shared, swiglu_limit: float) -> torch.Tensor
     return sd(h2)
 
 
+def _moe_layer_mxfp4(x, idx, w, gate, up, down, swiglu_limit, shared, expert_base, out_f32, few_token_path):
+    """moe_layer over MXFP4 experts: the same two paths and the same order of operations."""
+    lib = _lib.load()
+    dev = _lib.require_cuda(x, idx, w, gate.weight, up.weight, down.weight)
+    if x.dim() != 2 or idx.dim() != 2 or idx.shape[0] != x.shape[0] or w.shape != idx.shape:
+        raise JangqError(_lib.JQ_EINVAL, f"moe_layer: x [T, H], idx and w [T, k], got {tuple(x.shape)}, {tuple(idx.shape)}, "
+                                         f"{tuple(w.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise JangqError(_lib.JQ_EINVAL, f"activations must be bfloat16 or float16, got {x.dtype}")
+    if (gate.E, gate.N, gate.K) != (up.E, up.N, up.K) or down.E != gate.E or gate.K != x.shape[1] or down.K != gate.N:
+        raise JangqError(_lib.JQ_EINVAL, "moe_layer: gate and up are [E, I, H], down is [E, H, I]")
+    T, H = x.shape
+    k = idx.shape[1]
+    P, I = T * k, gate.N
+    if T == 0:
+        return torch.empty((0, down.N), dtype=torch.float32 if out_f32 else x.dtype, device=dev)
+    x = rows_ok(x)
+    idx32 = idx.reshape(-1).to(torch.int32).contiguous()
+    wf = w.reshape(-1).float().contiguous()
+    dt, st = _lib.dtype_id(x.dtype), _lib.stream_ptr(dev)
+    with _lib.on_device(dev):
+        use_sorted = P >= SORT_THRESHOLD if few_token_path is None else not few_token_path
+        h = torch.empty((P, I), dtype=x.dtype, device=dev)
+        if use_sorted and gate.gemm_ok and down.gemm_ok:
+            sp = SortedPairs(idx32, gate.E, expert_base, tile_m=_lib.MOE_GEMM_TILE_M)
+            xs = _gather_rows(x, sp, k)
+            _lib.check(lib.jq_mxfp4_moe_gate_up_swiglu(
+                xs.data_ptr(), dt, sp.n, xs.stride(0), sp.offsets.data_ptr(), sp.tile_expert.data_ptr(), sp.tile_row0.data_ptr(),
+                sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, gate.codes_tab.data_ptr(), gate.scales_tab.data_ptr(),
+                up.codes_tab.data_ptr(), up.scales_tab.data_ptr(), I, gate.K, wf.data_ptr(), sp.order.data_ptr(),
+                float(swiglu_limit), h.data_ptr(), h.stride(0), st))
+            y, inv = expert_gemm(h, sp, down), sp.inv.data_ptr()
+        else:
+            g, u = (expert_gemv(x, k, idx32, b, expert_base) for b in (gate, up))
+            _lib.check(lib.jq_moe_swiglu(g.data_ptr(), u.data_ptr(), g.stride(0), wf.data_ptr(), None, None, h.data_ptr(),
+                                         h.stride(0), I, P, float(swiglu_limit), dt, st))
+            y, inv = expert_gemv(h, 1, idx32, down, expert_base), None
+        ys = _shared_expert(x, shared, swiglu_limit) if shared is not None else None
+        out = torch.empty((T, down.N), dtype=torch.float32 if out_f32 else x.dtype, device=dev)
+        _lib.check(lib.jq_moe_combine_shared(y.data_ptr(), y.stride(0), inv, None, T, k, down.N,
+                                             ys.data_ptr() if ys is not None else None, ys.stride(0) if ys is not None else 0,
+                                             None if out_f32 else out.data_ptr(), down.N, out.data_ptr() if out_f32 else None,
+                                             dt, st))
+    return out
+
+
 def moe_layer(x: torch.Tensor, idx: torch.Tensor, w: torch.Tensor, gate: ExpertBank, up: ExpertBank,
               down: ExpertBank, swiglu_limit: float = 0.0, shared=None, expert_base: int = 0,
               out_f32: bool = False, all_local: bool | None = None, return_slots: bool = False,
@@ -393,7 +479,13 @@ def moe_layer(x: torch.Tensor, idx: torch.Tensor, w: torch.Tensor, gate: ExpertB
     the few-token mat-vecs may prefetch them while their predecessor still runs.  few_local says that most
     pairs name experts of other ranks (up to 128 pairs then stay on the integer gather).  few_token_path forces
     (True) or forbids (False) the unsorted gather mat-vec path; default: below 64 pairs, as the reference.
+    Banks of MXFP4 experts (MXFP4ExpertBank) are taken as well, all three or none; static_weights and few_local have no
+    meaning there, and return_slots is not provided.
     """
+    if any(isinstance(b, MXFP4ExpertBank) for b in (gate, up, down)):
+        if return_slots or not all(isinstance(b, MXFP4ExpertBank) for b in (gate, up, down)):
+            raise JangqError(_lib.JQ_EUNSUPPORTED, "moe_layer: MXFP4 banks come as gate, up and down, without return_slots")
+        return _moe_layer_mxfp4(x, idx, w, gate, up, down, swiglu_limit, shared, expert_base, out_f32, few_token_path)
     lib = _lib.load()
     dev = _lib.require_cuda(x, idx, w)
     T, H = x.shape

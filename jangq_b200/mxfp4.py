@@ -1,0 +1,235 @@
+"""Microscaled 4-bit floating point (OCP MXFP4) beside the affine codec: quantizer, products, experts' products.
+
+    mxfp4_quantize / mxfp4_dequantize   <-> quantize / dequantize
+    mxfp4_matmul                        <-> quantized_matmul; with x_scales both operands are MXFP4
+    mxfp4_gather_matmul, MXFP4ExpertBank <-> gather_qmm, ExpertBank
+
+A tensor is a pair: codes torch.int32 [.., K/8] (eight e2m1 numbers per word, the first in the lowest bits, the affine
+codec's 4-bit layout) and scales torch.uint8 [.., K/32], the power of two 2^(byte - 127) of 32 neighbouring numbers.
+The reference writes such bundles with its MXFP4 converters and runs them through mx.quantized_matmul.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import JangqError
+
+BLOCK = 32
+SORT_THRESHOLD = 64      # pairs; as gather_qmm
+
+
+def _check_pair(wq: torch.Tensor, scales: torch.Tensor, what: str = "codes"):
+    """int32 codes and uint8 scales of one shape, contiguous and aligned for the kernels -> (codes, scales, K)."""
+    if wq.dtype == torch.uint32:
+        wq = wq.view(torch.int32)
+    if wq.dtype != torch.int32 or scales.dtype != torch.uint8:
+        raise JangqError(_lib.JQ_EINVAL, f"{what} must be int32/uint32 and scales uint8, got {wq.dtype} and {scales.dtype}")
+    if wq.dim() < 1 or wq.shape[-1] == 0 or wq.shape[-1] % 4:
+        raise JangqError(_lib.JQ_EINVAL, f"{what} of shape {tuple(wq.shape)} do not hold whole blocks of {BLOCK}")
+    if scales.shape != wq.shape[:-1] + (wq.shape[-1] // 4,):
+        raise JangqError(_lib.JQ_EINVAL, f"scales shape {tuple(scales.shape)} does not match {what} {tuple(wq.shape)}: one byte "
+                                         f"per {BLOCK} numbers")
+    return _aligned(wq), _aligned(scales), wq.shape[-1] * 8
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def rows_ok(x: torch.Tensor) -> torch.Tensor:
+    """x [M, K] itself where the kernels take its rows (16-byte aligned, unit stride), else a copy."""
+    M, K = x.shape
+    if x.stride(1) == 1 and x.data_ptr() % 16 == 0:
+        if M == 1:           # the pitch of a single row is whatever the view it came from had and says nothing
+            return x if x.stride(0) == K else x.as_strided((1, K), (K, 1))
+        if x.stride(0) % 8 == 0 and x.stride(0) >= K:
+            return x
+    return _aligned(x)
+
+
+def mxfp4_quantize(w: torch.Tensor):
+    """MXFP4 along the last axis (a multiple of 32) -> (codes int32 [.., K/8], scales uint8 [.., K/32]).
+
+    Per 32 numbers the scale is 2^(floor(log2(max |w|)) - 2), not below 2^-127; numbers go to the nearest of
+    0 .5 1 1.5 2 3 4 6 times the scale, ties to the even code, 6 and above to 6.  A block with an infinity or a NaN gets
+    scale byte 255 and dequantizes to NaN.  w: float32, float16 or bfloat16."""
+    dev = _lib.require_cuda(w)
+    lib = _lib.load()
+    if w.dim() < 1 or w.shape[-1] % BLOCK or w.shape[-1] == 0:
+        raise JangqError(_lib.JQ_EINVAL, f"mxfp4_quantize expects rows of whole blocks of {BLOCK}, got {tuple(w.shape)}")
+    dt = _lib.dtype_id(w.dtype)
+    K = w.shape[-1]
+    w = _aligned(w)
+    lead = tuple(w.shape[:-1])
+    wq = torch.empty(lead + (K // 8,), dtype=torch.int32, device=dev)
+    scales = torch.empty(lead + (K // BLOCK,), dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(lib.jq_mxfp4_quantize(w.data_ptr(), dt, w.numel() // K, K, wq.data_ptr(), scales.data_ptr(),
+                                         _lib.stream_ptr(dev)))
+    return wq, scales
+
+
+def mxfp4_dequantize(wq: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The numbers a packed pair stands for -> [.., K], rounded once to `dtype` (exact in bfloat16 and float32)."""
+    dev = _lib.require_cuda(wq, scales)
+    lib = _lib.load()
+    wq, scales, K = _check_pair(wq, scales)
+    out = torch.empty(tuple(wq.shape[:-1]) + (K,), dtype=dtype, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(lib.jq_mxfp4_dequantize(wq.data_ptr(), scales.data_ptr(), out.numel() // K, K, out.data_ptr(),
+                                           _lib.dtype_id(dtype), _lib.stream_ptr(dev)))
+    return out
+
+
+def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scales: torch.Tensor | None = None,
+                 dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y[.., N] = x[.., K] . deq(w, scales)[N, K]^T with float32 sums.
+
+    x bfloat16 or float16: up to 16 rows run the mat-vec kernel, more the tensor-core GEMM; the output has x's type, and
+    the weight enters in it (exact in bfloat16; in float16 rounded once, and beyond 65504 infinite).
+    x int32 codes [.., K/8] with x_scales uint8 [.., K/32] (mxfp4_quantize of the activations): both operands go to the
+    tensor cores in 4 bits; the output type is `dtype` (bfloat16 by default)."""
+    dev = _lib.require_cuda(x, w, scales, x_scales)
+    lib = _lib.load()
+    w, scales, K = _check_pair(w, scales, "weight codes")
+    if w.dim() != 2:
+        raise JangqError(_lib.JQ_EINVAL, f"weight must be 2-D [N, K/8], got {tuple(w.shape)}")
+    N = w.shape[0]
+    if x_scales is not None:
+        x, x_scales, kx = _check_pair(x, x_scales, "activation codes")
+        if kx != K:
+            raise JangqError(_lib.JQ_EINVAL, f"x has {kx} features, weight expects {K}")
+        lead = tuple(x.shape[:-1])
+        M = x.numel() // (K // 8)
+        y = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=dev)
+        with _lib.on_device(dev):
+            _lib.check(lib.jq_mxfp4_gemm4(x.data_ptr(), x_scales.data_ptr(), M, w.data_ptr(), scales.data_ptr(), N, K,
+                                          y.data_ptr(), _lib.dtype_id(y.dtype), N, _lib.stream_ptr(dev)))
+        return y.reshape(lead + (N,))
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise JangqError(_lib.JQ_EINVAL, f"activations must be bfloat16 or float16 (or MXFP4 codes with x_scales), got {x.dtype}")
+    if dtype is not None and dtype != x.dtype:
+        raise JangqError(_lib.JQ_EUNSUPPORTED, f"the output of 16-bit activations has their type, {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise JangqError(_lib.JQ_EINVAL, f"x of shape {tuple(x.shape)} does not have the weight's {K} features")
+    lead = tuple(x.shape[:-1])
+    x2 = rows_ok(x if x.dim() == 2 else x.reshape(-1, K))
+    M, dt = x2.shape[0], _lib.dtype_id(x.dtype)
+    y = torch.empty((M, N), dtype=x.dtype, device=dev)
+    with _lib.on_device(dev):
+        st = _lib.stream_ptr(dev)
+        if M > _lib.QGEMV_MAX_M and K % 64 == 0:
+            _lib.check(lib.jq_mxfp4_gemm(x2.data_ptr(), dt, M, x2.stride(0), w.data_ptr(), scales.data_ptr(), N, K, y.data_ptr(), N, st))
+        else:
+            # an odd number of blocks is the mat-vec's, 16 rows at a time
+            for m0 in range(0, M, _lib.QGEMV_MAX_M):
+                rows = x2[m0:m0 + _lib.QGEMV_MAX_M]
+                _lib.check(lib.jq_mxfp4_gemv(rows.data_ptr(), dt, rows.shape[0], x2.stride(0), w.data_ptr(), scales.data_ptr(), N, K,
+                                             y[m0:].data_ptr(), N, st))
+    return y.reshape(lead + (N,))
+
+
+class MXFP4ExpertBank:
+    """MXFP4 weights of E experts for one projection: `weight` int32/uint32 [E, N, K/8], `scales` uint8 [E, N, K/32].
+    Device pointer tables for the grouped products are built once."""
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor):
+        self.device = _lib.require_cuda(weight, scales)
+        if weight.dim() != 3:
+            raise JangqError(_lib.JQ_EINVAL, f"stacked expert weight must be [E, N, K/8], got {tuple(weight.shape)}")
+        self.weight, self.scales, self.K = _check_pair(weight, scales, "expert codes")
+        self.E, self.N = self.weight.shape[:2]
+        wstep, sstep = self.N * self.K // 2, self.N * self.K // BLOCK
+        if self.E < 1 or self.N < 1:
+            raise JangqError(_lib.JQ_EINVAL, f"a bank holds at least one row of one expert, got {tuple(weight.shape)}")
+        experts = torch.arange(self.E, dtype=torch.int64, device=self.device)
+        self.codes_tab = self.weight.data_ptr() + experts * wstep
+        self.scales_tab = self.scales.data_ptr() + experts * sstep
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor) -> "MXFP4ExpertBank":
+        """Quantize float experts [E, N, K] on the GPU (mxfp4_quantize)."""
+        return cls(*mxfp4_quantize(w))
+
+    @property
+    def gemm_ok(self) -> bool:
+        """Shapes the tensor-core grouped product takes."""
+        return self.K % 64 == 0
+
+
+def expert_gemv(x: torch.Tensor, x_div: int, pair_expert: torch.Tensor, bank: MXFP4ExpertBank, expert_base: int = 0) -> torch.Tensor:
+    """y[p] = deq(W[pair_expert[p] - expert_base]) . x[p // x_div], one mat-vec per pair; rows of experts outside the bank
+    are zero."""
+    lib = _lib.load()
+    P = pair_expert.numel()
+    y = torch.empty((P, bank.N), dtype=x.dtype, device=x.device)
+    step = max(1, 32768 // x_div) * x_div             # pairs of one launch, those of whole tokens
+    for p0 in range(0, P, step):
+        n = min(step, P - p0)
+        _lib.check(lib.jq_mxfp4_gather_gemv(x[p0 // x_div:].data_ptr(), _lib.dtype_id(x.dtype), x.stride(0), x_div,
+                                            pair_expert[p0:].data_ptr(), n, bank.weight.data_ptr(), bank.scales.data_ptr(), bank.E,
+                                            expert_base, bank.N, bank.K, y[p0:].data_ptr(), bank.N, _lib.stream_ptr(x.device)))
+    return y
+
+
+def expert_gemm(x_sorted: torch.Tensor, sp, bank: MXFP4ExpertBank) -> torch.Tensor:
+    """The grouped product over expert-sorted rows (moe.SortedPairs)."""
+    lib = _lib.load()
+    y = torch.empty((x_sorted.shape[0], bank.N), dtype=x_sorted.dtype, device=x_sorted.device)
+    _lib.check(lib.jq_mxfp4_moe_gemm(x_sorted.data_ptr(), _lib.dtype_id(x_sorted.dtype), sp.n, x_sorted.stride(0),
+                                     sp.offsets.data_ptr(), sp.tile_expert.data_ptr(), sp.tile_row0.data_ptr(),
+                                     sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, bank.codes_tab.data_ptr(),
+                                     bank.scales_tab.data_ptr(), bank.N, bank.K, y.data_ptr(), bank.N,
+                                     _lib.stream_ptr(x_sorted.device)))
+    return y
+
+
+def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, rhs_indices: torch.Tensor | None = None,
+                        lhs_indices: torch.Tensor | None = None, sorted_indices: bool = False) -> torch.Tensor:
+    """y[r] = x[lhs[r]] . deq(w[rhs[r]])^T for stacked MXFP4 experts w [E, N, K/8], scales [E, N, K/32] (or an
+    MXFP4ExpertBank): gather_qmm's call shape, indices and result [R, N] (x [R0, K]; rhs_indices [R] or [T, k]; without
+    lhs_indices row r of x is used when R0 == R, row r // k when rhs is [T, k] with R0 == T).  Indices outside the bank
+    give rows of zeros.  Below 64 rows one mat-vec per row, above that the grouped tensor-core product."""
+    if rhs_indices is None:
+        raise JangqError(_lib.JQ_EINVAL, "mxfp4_gather_matmul needs rhs_indices")
+    if sorted_indices and lhs_indices is None:
+        raise ValueError("sorted_indices=True requires lhs_indices")
+    if not isinstance(w, MXFP4ExpertBank) and scales is None:
+        raise JangqError(_lib.JQ_EINVAL, "mxfp4_gather_matmul needs scales with stacked codes")
+    bank = w if isinstance(w, MXFP4ExpertBank) else MXFP4ExpertBank(w, scales)
+    dev = _lib.require_cuda(x, rhs_indices, lhs_indices, bank.weight)
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise JangqError(_lib.JQ_EINVAL, f"activations must be bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != bank.K:
+        raise JangqError(_lib.JQ_EINVAL, f"x of shape {tuple(x.shape)} does not have the experts' {bank.K} features")
+    x2 = x if x.dim() == 2 else x.reshape(-1, bank.K)
+    k = rhs_indices.shape[-1] if rhs_indices.dim() == 2 else 1
+    rhs = rhs_indices.reshape(-1).to(torch.int32).contiguous()
+    R = rhs.numel()
+    if lhs_indices is not None:
+        lhs = lhs_indices.reshape(-1).to(torch.int64)
+        if lhs.numel() != R:
+            raise JangqError(_lib.JQ_EINVAL, "lhs_indices and rhs_indices differ in length")
+        x2, x_div = x2.index_select(0, lhs), 1
+    elif x2.shape[0] == R:
+        x_div = 1
+    elif rhs_indices.dim() == 2 and x2.shape[0] == rhs_indices.shape[0]:
+        x_div = k
+    else:
+        raise JangqError(_lib.JQ_EINVAL, f"cannot match {x2.shape[0]} rows of x with {R} indices")
+    if R == 0:
+        return torch.empty((0, bank.N), dtype=x.dtype, device=dev)
+    x2 = rows_ok(x2)
+    with _lib.on_device(dev):
+        if R < SORT_THRESHOLD or not bank.gemm_ok:
+            return expert_gemv(x2, x_div, rhs, bank)
+        from . import moe
+        sp = moe.SortedPairs(rhs, bank.E, tile_m=_lib.MOE_GEMM_TILE_M)
+        ys = expert_gemm(moe._gather_rows(x2, sp, x_div), sp, bank)
+        y = torch.empty((R, bank.N), dtype=x.dtype, device=dev)
+        # back to the order of the pairs; pairs without an expert of the bank have no row and get zeros
+        _lib.check(_lib.load().jq_moe_combine_shared(ys.data_ptr(), ys.stride(0), sp.inv.data_ptr(), None, R, 1, bank.N, None, 0,
+                                                     y.data_ptr(), bank.N, None, _lib.dtype_id(x.dtype), _lib.stream_ptr(dev)))
+        return y
