@@ -302,8 +302,8 @@ def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch
     if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
         logits = logits.contiguous()
     # sizes a table cannot have are refused by the library; nothing of theirs is allocated before
-    idx = torch.empty((T, max(k, 0)), dtype=torch.int32, device=dev)
-    w = torch.empty((T, max(k, 0)), dtype=torch.float32, device=dev)
+    idx = logits.new_empty((T, max(k, 0)), dtype=torch.int32)
+    w = logits.new_empty((T, max(k, 0)), dtype=torch.float32)
     with _lib.on_device(dev):
         _lib.check(lib.jq_moe_route_topk(logits.data_ptr(), _lib.dtype_id(logits.dtype), logits.stride(0) if T > 1 else E, T, E,
                                          k, _SCORES[score], bias.data_ptr() if bias is not None else None, groups, groups_kept,

@@ -19,18 +19,27 @@ BLOCK = 32
 SORT_THRESHOLD = 64      # pairs; as gather_qmm
 
 
+# A small product is a few microseconds of kernel, so the checks below take the short way where there is one: no slices and
+# no reshapes that change nothing, and new_empty, which is cheaper than torch.empty with a device.
+
 def _check_pair(wq: torch.Tensor, scales: torch.Tensor, what: str = "codes"):
     """int32 codes and uint8 scales of one shape, contiguous and aligned for the kernels -> (codes, scales, K)."""
-    if wq.dtype == torch.uint32:
+    if wq.dtype is torch.uint32:
         wq = wq.view(torch.int32)
-    if wq.dtype != torch.int32 or scales.dtype != torch.uint8:
+    if wq.dtype is not torch.int32 or scales.dtype is not torch.uint8:
         raise JangqError(_lib.JQ_EINVAL, f"{what} must be int32/uint32 and scales uint8, got {wq.dtype} and {scales.dtype}")
-    if wq.dim() < 1 or wq.shape[-1] == 0 or wq.shape[-1] % 4:
-        raise JangqError(_lib.JQ_EINVAL, f"{what} of shape {tuple(wq.shape)} do not hold whole blocks of {BLOCK}")
-    if scales.shape != wq.shape[:-1] + (wq.shape[-1] // 4,):
-        raise JangqError(_lib.JQ_EINVAL, f"scales shape {tuple(scales.shape)} does not match {what} {tuple(wq.shape)}: one byte "
+    shape = wq.shape
+    words = shape[-1] if shape else 0
+    if words == 0 or words % 4:
+        raise JangqError(_lib.JQ_EINVAL, f"{what} of shape {tuple(shape)} do not hold whole blocks of {BLOCK}")
+    if scales.shape != shape[:-1] + (words // 4,):
+        raise JangqError(_lib.JQ_EINVAL, f"scales shape {tuple(scales.shape)} does not match {what} {tuple(shape)}: one byte "
                                          f"per {BLOCK} numbers")
-    return _aligned(wq), _aligned(scales), wq.shape[-1] * 8
+    if not wq.is_contiguous() or wq.data_ptr() % 16:
+        wq = _aligned(wq)
+    if not scales.is_contiguous() or scales.data_ptr() % 16:
+        scales = _aligned(scales)
+    return wq, scales, words * 8
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -61,10 +70,11 @@ def mxfp4_quantize(w: torch.Tensor):
         raise JangqError(_lib.JQ_EINVAL, f"mxfp4_quantize expects rows of whole blocks of {BLOCK}, got {tuple(w.shape)}")
     dt = _lib.dtype_id(w.dtype)
     K = w.shape[-1]
-    w = _aligned(w)
-    lead = tuple(w.shape[:-1])
-    wq = torch.empty(lead + (K // 8,), dtype=torch.int32, device=dev)
-    scales = torch.empty(lead + (K // BLOCK,), dtype=torch.uint8, device=dev)
+    if not w.is_contiguous() or w.data_ptr() % 16:
+        w = _aligned(w)
+    lead = w.shape[:-1]
+    wq = w.new_empty(lead + (K // 8,), dtype=torch.int32)
+    scales = w.new_empty(lead + (K // BLOCK,), dtype=torch.uint8)
     with _lib.on_device(dev):
         _lib.check(lib.jq_mxfp4_quantize(w.data_ptr(), dt, w.numel() // K, K, wq.data_ptr(), scales.data_ptr(),
                                          _lib.stream_ptr(dev)))
@@ -76,7 +86,7 @@ def mxfp4_dequantize(wq: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
     dev = _lib.require_cuda(wq, scales)
     lib = _lib.load()
     wq, scales, K = _check_pair(wq, scales)
-    out = torch.empty(tuple(wq.shape[:-1]) + (K,), dtype=dtype, device=dev)
+    out = wq.new_empty(wq.shape[:-1] + (K,), dtype=dtype)
     with _lib.on_device(dev):
         _lib.check(lib.jq_mxfp4_dequantize(wq.data_ptr(), scales.data_ptr(), out.numel() // K, K, out.data_ptr(),
                                            _lib.dtype_id(dtype), _lib.stream_ptr(dev)))
@@ -101,34 +111,34 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
         x, x_scales, kx = _check_pair(x, x_scales, "activation codes")
         if kx != K:
             raise JangqError(_lib.JQ_EINVAL, f"x has {kx} features, weight expects {K}")
-        lead = tuple(x.shape[:-1])
-        M = x.numel() // (K // 8)
-        y = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=dev)
+        y = x.new_empty(x.shape[:-1] + (N,), dtype=dtype or torch.bfloat16)
         with _lib.on_device(dev):
-            _lib.check(lib.jq_mxfp4_gemm4(x.data_ptr(), x_scales.data_ptr(), M, w.data_ptr(), scales.data_ptr(), N, K,
-                                          y.data_ptr(), _lib.dtype_id(y.dtype), N, _lib.stream_ptr(dev)))
-        return y.reshape(lead + (N,))
-    if x.dtype not in (torch.bfloat16, torch.float16):
+            _lib.check(lib.jq_mxfp4_gemm4(x.data_ptr(), x_scales.data_ptr(), x.numel() // (K // 8), w.data_ptr(),
+                                          scales.data_ptr(), N, K, y.data_ptr(), _lib.dtype_id(y.dtype), N, _lib.stream_ptr(dev)))
+        return y
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
         raise JangqError(_lib.JQ_EINVAL, f"activations must be bfloat16 or float16 (or MXFP4 codes with x_scales), got {x.dtype}")
     if dtype is not None and dtype != x.dtype:
         raise JangqError(_lib.JQ_EUNSUPPORTED, f"the output of 16-bit activations has their type, {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise JangqError(_lib.JQ_EINVAL, f"x of shape {tuple(x.shape)} does not have the weight's {K} features")
-    lead = tuple(x.shape[:-1])
-    x2 = rows_ok(x if x.dim() == 2 else x.reshape(-1, K))
-    M, dt = x2.shape[0], _lib.dtype_id(x.dtype)
-    y = torch.empty((M, N), dtype=x.dtype, device=dev)
+    xshape = x.shape
+    if not xshape or xshape[-1] != K:
+        raise JangqError(_lib.JQ_EINVAL, f"x of shape {tuple(xshape)} does not have the weight's {K} features")
+    y = x.new_empty(xshape[:-1] + (N,))
+    x2 = rows_ok(x if len(xshape) == 2 else x.reshape(-1, K))
+    M, ld = x2.shape[0], x2.stride(0)
+    dt, xp, yp, wp, sp = _lib.dtype_id(x.dtype), x2.data_ptr(), y.data_ptr(), w.data_ptr(), scales.data_ptr()
     with _lib.on_device(dev):
         st = _lib.stream_ptr(dev)
-        if M > _lib.QGEMV_MAX_M and K % 64 == 0:
-            _lib.check(lib.jq_mxfp4_gemm(x2.data_ptr(), dt, M, x2.stride(0), w.data_ptr(), scales.data_ptr(), N, K, y.data_ptr(), N, st))
+        if M <= _lib.QGEMV_MAX_M:
+            _lib.check(lib.jq_mxfp4_gemv(xp, dt, M, ld, wp, sp, N, K, yp, N, st))
+        elif K % 64 == 0:
+            _lib.check(lib.jq_mxfp4_gemm(xp, dt, M, ld, wp, sp, N, K, yp, N, st))
         else:
             # an odd number of blocks is the mat-vec's, 16 rows at a time
             for m0 in range(0, M, _lib.QGEMV_MAX_M):
-                rows = x2[m0:m0 + _lib.QGEMV_MAX_M]
-                _lib.check(lib.jq_mxfp4_gemv(rows.data_ptr(), dt, rows.shape[0], x2.stride(0), w.data_ptr(), scales.data_ptr(), N, K,
-                                             y[m0:].data_ptr(), N, st))
-    return y.reshape(lead + (N,))
+                _lib.check(lib.jq_mxfp4_gemv(xp + 2 * m0 * ld, dt, min(_lib.QGEMV_MAX_M, M - m0), ld, wp, sp, N, K,
+                                             yp + 2 * m0 * N, N, st))
+    return y
 
 
 class MXFP4ExpertBank:
@@ -164,20 +174,21 @@ def expert_gemv(x: torch.Tensor, x_div: int, pair_expert: torch.Tensor, bank: MX
     are zero."""
     lib = _lib.load()
     P = pair_expert.numel()
-    y = torch.empty((P, bank.N), dtype=x.dtype, device=x.device)
+    N, K, ld = bank.N, bank.K, x.stride(0)
+    y = x.new_empty((P, N))
+    dt, xp, ip, yp = _lib.dtype_id(x.dtype), x.data_ptr(), pair_expert.data_ptr(), y.data_ptr()
+    wp, sp, st = bank.weight.data_ptr(), bank.scales.data_ptr(), _lib.stream_ptr(x.device)
     step = max(1, 32768 // x_div) * x_div             # pairs of one launch, those of whole tokens
     for p0 in range(0, P, step):
-        n = min(step, P - p0)
-        _lib.check(lib.jq_mxfp4_gather_gemv(x[p0 // x_div:].data_ptr(), _lib.dtype_id(x.dtype), x.stride(0), x_div,
-                                            pair_expert[p0:].data_ptr(), n, bank.weight.data_ptr(), bank.scales.data_ptr(), bank.E,
-                                            expert_base, bank.N, bank.K, y[p0:].data_ptr(), bank.N, _lib.stream_ptr(x.device)))
+        _lib.check(lib.jq_mxfp4_gather_gemv(xp + 2 * (p0 // x_div) * ld, dt, ld, x_div, ip + 4 * p0, min(step, P - p0), wp, sp,
+                                            bank.E, expert_base, N, K, yp + 2 * p0 * N, N, st))
     return y
 
 
 def expert_gemm(x_sorted: torch.Tensor, sp, bank: MXFP4ExpertBank) -> torch.Tensor:
     """The grouped product over expert-sorted rows (moe.SortedPairs)."""
     lib = _lib.load()
-    y = torch.empty((x_sorted.shape[0], bank.N), dtype=x_sorted.dtype, device=x_sorted.device)
+    y = x_sorted.new_empty((x_sorted.shape[0], bank.N))
     _lib.check(lib.jq_mxfp4_moe_gemm(x_sorted.data_ptr(), _lib.dtype_id(x_sorted.dtype), sp.n, x_sorted.stride(0),
                                      sp.offsets.data_ptr(), sp.tile_expert.data_ptr(), sp.tile_row0.data_ptr(),
                                      sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, bank.codes_tab.data_ptr(),
@@ -206,8 +217,10 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
         raise JangqError(_lib.JQ_EINVAL, f"x of shape {tuple(x.shape)} does not have the experts' {bank.K} features")
     x2 = x if x.dim() == 2 else x.reshape(-1, bank.K)
     k = rhs_indices.shape[-1] if rhs_indices.dim() == 2 else 1
-    rhs = rhs_indices.reshape(-1).to(torch.int32).contiguous()
-    R = rhs.numel()
+    R = rhs_indices.numel()
+    rhs = rhs_indices
+    if rhs.dtype is not torch.int32 or not rhs.is_contiguous():
+        rhs = rhs.to(torch.int32).contiguous()
     if lhs_indices is not None:
         lhs = lhs_indices.reshape(-1).to(torch.int64)
         if lhs.numel() != R:
@@ -215,12 +228,12 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
         x2, x_div = x2.index_select(0, lhs), 1
     elif x2.shape[0] == R:
         x_div = 1
-    elif rhs_indices.dim() == 2 and x2.shape[0] == rhs_indices.shape[0]:
+    elif rhs_indices.dim() == 2 and x2.shape[0] == rhs_indices.shape[0] and k > 0:
         x_div = k
     else:
         raise JangqError(_lib.JQ_EINVAL, f"cannot match {x2.shape[0]} rows of x with {R} indices")
     if R == 0:
-        return torch.empty((0, bank.N), dtype=x.dtype, device=dev)
+        return x.new_empty((0, bank.N))
     x2 = rows_ok(x2)
     with _lib.on_device(dev):
         if R < SORT_THRESHOLD or not bank.gemm_ok:
@@ -228,7 +241,7 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
         from . import moe
         sp = moe.SortedPairs(rhs, bank.E, tile_m=_lib.MOE_GEMM_TILE_M)
         ys = expert_gemm(moe._gather_rows(x2, sp, x_div), sp, bank)
-        y = torch.empty((R, bank.N), dtype=x.dtype, device=dev)
+        y = x.new_empty((R, bank.N))
         # back to the order of the pairs; pairs without an expert of the bank have no row and get zeros
         _lib.check(_lib.load().jq_moe_combine_shared(ys.data_ptr(), ys.stride(0), sp.inv.data_ptr(), None, R, 1, bank.N, None, 0,
                                                      y.data_ptr(), bank.N, None, _lib.dtype_id(x.dtype), _lib.stream_ptr(dev)))
