@@ -520,7 +520,9 @@ int jq_mxfp4_dequantize(const uint32_t* codes, const uint8_t* scales, int64_t ro
  * jq_mxfp4_gather_gemv: y[p] = x[p / x_div] . deq(w[pair_expert[p] - expert_base])^T for the pairs of routed experts; codes
  *   [num_experts, N, K/8] and scales [num_experts, N, K/32] are stacked; pairs of other experts get rows of zeros.
  * jq_mxfp4_moe_gemm, jq_mxfp4_moe_gate_up_swiglu: jq_moe_gemm_tiled and jq_moe_gate_up_swiglu over MXFP4 experts (tile
- *   lists of 128 or 192 rows, pointer tables to codes and scales, which must be 16- and 2-byte aligned).
+ *   lists of 128 or 192 rows, pointer tables to codes and scales, which must be 16- and 2-byte aligned).  With order and
+ *   inv of jq_moe_sort (both or neither) jq_mxfp4_moe_gemm stores its rows where the pairs stand, y[order[r]], and zeroes
+ *   the rows of pairs that no expert of the bank took (inv < 0; max_rows is then the number of pairs).
  * jq_mxfp4_gemm4: both operands in MXFP4 on the block-scaled tensor-core path, y f32, f16 or bf16; any M, K % 32 == 0. */
 int jq_mxfp4_gemv(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint32_t* codes, const uint8_t* scales,
                   int64_t N, int64_t K, void* y, int64_t ldy, jq_stream_t stream);
@@ -532,7 +534,7 @@ int jq_mxfp4_gather_gemv(const void* x, int x_dtype, int64_t ldx, int x_div, con
 int jq_mxfp4_moe_gemm(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx, const int32_t* expert_offsets,
                       const int32_t* tile_expert, const int32_t* tile_row0, const int32_t* num_tiles, int64_t max_tiles,
                       int tile_m, const uint32_t* const* codes_tab, const uint8_t* const* scales_tab, int64_t N, int64_t K,
-                      void* y_sorted, int64_t ldy, jq_stream_t stream);
+                      const int32_t* order, const int32_t* inv, void* y, int64_t ldy, jq_stream_t stream);
 int jq_mxfp4_moe_gate_up_swiglu(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx,
                                 const int32_t* expert_offsets, const int32_t* tile_expert, const int32_t* tile_row0,
                                 const int32_t* num_tiles, int64_t max_tiles, int tile_m, const uint32_t* const* gate_codes,

@@ -116,7 +116,7 @@ SIGNATURES = {
     "jq_mxfp4_gemv": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p]),
     "jq_mxfp4_gemm": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p]),
     "jq_mxfp4_gather_gemv": (C.c_int, [_p, _i32, _i64, _i32, _p, _i64, _p, _p, _i32, _i32, _i64, _i64, _p, _i64, _p]),
-    "jq_mxfp4_moe_gemm": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _p, _p, _i64, _i64, _p, _i64, _p]),
+    "jq_mxfp4_moe_gemm": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _p, _p, _i64, _i64, _p, _p, _p, _i64, _p]),
     "jq_mxfp4_moe_gate_up_swiglu": (C.c_int, [_p, _i32, _i64, _i64, _p, _p, _p, _p, _i64, _i32, _p, _p, _p, _p, _i64, _i64, _p,
                                               _p, C.c_float, _p, _i64, _p]),
     "jq_mxfp4_gemm4": (C.c_int, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _i32, _i64, _p]),

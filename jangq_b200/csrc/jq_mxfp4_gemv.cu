@@ -2,8 +2,8 @@
 // same for the (token, slot) pairs of routed experts.
 //
 // Bound: the weights' 17/32 byte each from HBM on paper; at 2 weights per byte the issue of their expansion is about as
-// long.  Warp MMAs (m16n8k16) with the weights as the 16-row operand: eight codes of a word become four pairs with one
-// multiply each (jq_mxfp4.cuh), the block's scale inside it, so every product of the row goes into one f32 accumulator.
+// long.  Warp MMAs (m16n8k16) with the weights as the 16-row operand: eight codes of a word become four pairs by byte
+// permutes over the block's scaled magnitudes (MxTable), so every product of the row goes into one f32 accumulator.
 // The sum over k does not care which k an MMA slot stands for: a lane takes two whole blocks (32 consecutive bytes) of
 // its row, and the activations are read in the same order.  A CTA owns 16 weight rows; its warps take every eighth
 // stretch of 256 codes and their sums meet in shared memory in warp order, so results do not depend on timing.
@@ -103,28 +103,24 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
         const bool fast = __all_sync(0xFFFFFFFFu, max(max(v0.s & 255u, v0.s >> 8), max(v1.s & 255u, v1.s >> 8)) <= Mx<AT>::FAST_MAX);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t b0 = h ? v0.s >> 8 : v0.s & 255u, b1 = h ? v1.s >> 8 : v1.s & 255u;
-            const uint32_t l0 = Mx<AT>::lift(b0), l1 = Mx<AT>::lift(b1);
+            MxTable<AT> t0, t1;
+            t0.build(h ? v0.s >> 8 : v0.s & 255u, fast);
+            t1.build(h ? v1.s >> 8 : v1.s & 255u, fast);
             const uint32_t q0[4] = {v0.q[h].x, v0.q[h].y, v0.q[h].z, v0.q[h].w};
             const uint32_t q1[4] = {v1.q[h].x, v1.q[h].y, v1.q[h].z, v1.q[h].w};
             const bool in = at + h < a.nblk;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t e0[4], e1[4];
-                if (fast) {
-                    mx_expand8<AT>(q0[j], l0, e0);
-                    mx_expand8<AT>(q1[j], l1, e1);
-                } else {
-                    mx_expand8_any<AT>(q0[j], b0, e0);
-                    mx_expand8_any<AT>(q1[j], b1, e1);
-                }
+                t0.expand(q0[j], e0);
+                t1.expand(q1[j], e1);
                 const uint32_t fa[4] = {e0[0], e1[0], e0[1], e1[1]}, fb[4] = {e0[2], e1[2], e0[3], e1[3]};
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     uint4 xv = make_uint4(0u, 0u, 0u, 0u);
                     if (live[i] && in) xv = *reinterpret_cast<const uint4*>(xr[i] + (at + h) * 32 + j * 8);
-                    A::mma(acc[i], fa, prmt(xv.x, xv.z, 0x5410), prmt(xv.x, xv.z, 0x7632));
-                    A::mma(acc[i], fb, prmt(xv.y, xv.w, 0x5410), prmt(xv.y, xv.w, 0x7632));
+                    A::mma(acc[i], fa, xv.x, xv.y);
+                    A::mma(acc[i], fb, xv.z, xv.w);
                 }
             }
         }

@@ -75,6 +75,9 @@ struct GemmArgs {
     const float* wts;
     const int32_t* order;
     float lim;
+    // scatter mode (SC): row r of the tiles is stored as row order[r] of y, and rows p of y with inv[p] < 0 (pairs without an
+    // expert of the bank, 0 <= p < M) are zeroed
+    const int32_t* inv;
 };
 
 // Scales and biases of one weight row: from the staged chunk (jq_ts.cuh), or, where rows are not staged, loaded one
@@ -164,16 +167,10 @@ __device__ __forceinline__ void expand_block_mx(const uint8_t* crow, int r, int 
     for (int h = 0; h < 2; ++h) {
         const uint4 v = cp[code_chunk<CPR>(kbi * 2 + h, r)];
         const uint32_t cur[4] = {v.x, v.y, v.z, v.w};
-        const uint32_t byte = h ? sb >> 8 : sb & 255u, lift = Mx<AT>::lift(byte);
+        MxTable<AT> table;
+        table.build(h ? sb >> 8 : sb & 255u, fast);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t f[4];                                   // codes (j, j + 4)
-            if (fast) mx_expand8<AT>(cur[i], lift, f);
-            else mx_expand8_any<AT>(cur[i], byte, f);
-            uint32_t* o = out + 16 * h + 4 * i;
-            o[0] = prmt(f[0], f[1], 0x5410); o[1] = prmt(f[2], f[3], 0x5410);
-            o[2] = prmt(f[0], f[1], 0x7632); o[3] = prmt(f[2], f[3], 0x7632);
-        }
+        for (int i = 0; i < 4; ++i) table.expand(cur[i], out + 16 * h + 4 * i);
     }
 }
 
@@ -199,6 +196,44 @@ __device__ __forceinline__ void store_columns(const GemmArgs& a, const uint32_t 
 #pragma unroll
         for (int j = 0; j < 32; ++j)
             if (j < rows) yb[j * a.ldy + nn] = A::from_f32(__uint_as_float(v[j]));
+    }
+}
+
+// the same, to the rows that the lanes hold: lane j's `to` is the row of y of column j
+template <typename AT>
+__device__ __forceinline__ void scatter_columns(const GemmArgs& a, const uint32_t (&v)[32], int to, int rows, int64_t nn, bool whole,
+                                                int lane) {
+    using A = Act<AT>;
+    uint16_t* yb = reinterpret_cast<uint16_t*>(a.y);
+    if (a.y_pair_ok && whole) {
+        const int odd = lane & 1;
+        uint16_t* yl = yb + (nn & ~1ll);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            const float keep = __uint_as_float(odd ? v[j + 1] : v[j]);
+            const float got = __uint_as_float(__shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1));
+            const int row = __shfl_sync(0xFFFFFFFFu, to, j + odd);
+            const uint32_t pk = odd ? A::pack_hi(got, keep) : A::pack_hi(keep, got);
+            if (j + odd < rows) *reinterpret_cast<uint32_t*>(yl + row * a.ldy) = pk;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const int row = __shfl_sync(0xFFFFFFFFu, to, j);
+            if (j < rows && nn < a.N) yb[row * a.ldy + nn] = A::from_f32(__uint_as_float(v[j]));
+        }
+    }
+}
+
+// rows of y without a result: the grid's warps look at 32 pairs at a time
+__device__ __forceinline__ void zero_missing_rows(const GemmArgs& a) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    for (int64_t p0 = ((int64_t)blockIdx.x * warps + (threadIdx.x >> 5)) * 32; p0 < a.M; p0 += (int64_t)gridDim.x * warps * 32) {
+        uint32_t missing = __ballot_sync(0xFFFFFFFFu, p0 + lane < a.M && a.inv[p0 + lane] < 0);
+        for (; missing; missing &= missing - 1) {
+            uint16_t* row = reinterpret_cast<uint16_t*>(a.y) + (p0 + __ffs(missing) - 1) * a.ldy;
+            for (int64_t n = lane; n < a.N; n += 32) row[n] = 0;
+        }
     }
 }
 
@@ -504,7 +539,7 @@ template <bool GU> __device__ __forceinline__ int pers_side_mode(const GemmArgs&
     return m == 0 || m2 == 0 ? 0 : max(m, m2);               // the copy that both matrices are aligned for
 }
 
-template <typename AT, int BITS, bool GU, int TN, bool MX = false>
+template <typename AT, int BITS, bool GU, int TN, bool MX = false, bool SC = false>
 __global__ void __launch_bounds__(PersCfg<BITS, TN>::THREADS, 1)
 qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
     using C = PersCfg<BITS, TN>;
@@ -527,6 +562,7 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
     const int nx = (int)((a.N + (GU ? 63 : 127)) / (GU ? 64 : 128));
     const int total = nx * min(*a.num_tiles, a.max_tiles);
     const int first = blockIdx.x, step = gridDim.x;
+    if constexpr (SC) zero_missing_rows(a);
     if (first >= total) return;              // uniform for the CTA, before any barrier or tensor-memory allocation
 
     if (threadIdx.x == 0) {
@@ -629,6 +665,10 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
                 float* wt = reinterpret_cast<float*>(smem + C::WT_OFF);
                 for (int q = r; q < t.rows; q += 128) wt[q] = a.wts ? a.wts[a.order[t.m0 + q]] : 1.0f;
             }
+            int to[SC ? C::TNMAX / 32 : 1];                  // where the tile's rows go, read while the MMAs run
+            if constexpr (SC)
+#pragma unroll
+                for (int i = 0; i < C::TNMAX / 32; ++i) to[i] = i * 32 + lane < t.rows ? a.order[t.m0 + i * 32 + lane] : 0;
             ok = __all_sync(0xFFFFFFFFu, ts_wait(accfull + d, dph));
             if constexpr (GU) {      // the four warps meet in barriers below: they go on or leave together
                 int all;
@@ -663,6 +703,11 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
                         store_swiglu<AT>(a, g4, u4, reinterpret_cast<const float*>(smem + C::WT_OFF)[c0 + tok], row, t.n0 + nl);
                     }
                     asm volatile("bar.sync 1, 128;" ::: "memory");
+                } else if constexpr (SC) {
+                    int here = to[0];
+#pragma unroll
+                    for (int i = 1; i < C::TNMAX / 32; ++i) here = c0 == i * 32 ? to[i] : here;
+                    scatter_columns<AT>(a, v, here, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane);
                 } else {
                     store_columns<AT>(a, v, t.m0 + c0, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane);
                 }
@@ -786,11 +831,11 @@ static int launch_gemm(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_til
     return check_launch("qgemm");
 }
 
-template <typename AT, int BITS, bool GU, int TN, bool MX = false>
+template <typename AT, int BITS, bool GU, int TN, bool MX = false, bool SC = false>
 static int launch_pers(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_tiles, cudaStream_t st) {
     using C = PersCfg<BITS, TN>;
     static_assert(C::SMEM <= GEMM_SMEM, "shared memory of one CTA");
-    auto kernel = qgemm_pers_kernel<AT, BITS, GU, TN, MX>;
+    auto kernel = qgemm_pers_kernel<AT, BITS, GU, TN, MX, SC>;
     static bool attr_done[64] = {};
     int dev = 0;
     JQ_CUDA_OK(cudaGetDevice(&dev));
@@ -819,6 +864,7 @@ struct GroupedArgs {
     const float* wts = nullptr;
     const int32_t* order = nullptr;
     float lim = 0.f;
+    const int32_t* inv = nullptr;      // scatter mode, with order
 };
 
 // Dense when grp == nullptr (codes/scales/biases of one matrix); grouped otherwise (x holds the M
@@ -868,7 +914,9 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
     a.scales_tab2 = gu ? grp->scales_tab2 : nullptr;
     a.biases_tab2 = gu ? grp->biases_tab2 : nullptr;
     a.wts = gu ? grp->wts : nullptr;
-    a.order = gu ? grp->order : nullptr;
+    const bool sc = grp && grp->inv;
+    a.order = gu || sc ? grp->order : nullptr;
+    a.inv = sc ? grp->inv : nullptr;
     a.lim = gu ? grp->lim : 0.f;
     int ks = 1;
     int64_t m_tiles;
@@ -927,6 +975,7 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
 #define JQ_GEMM_MX(T)                                                                                     \
     {                                                                                                     \
         if (gu) return launch_pers<T, 4, true, 192, true>(xmap, a, m_tiles, st);                          \
+        if (sc) return launch_pers<T, 4, false, 192, true, true>(xmap, a, m_tiles, st);                   \
         if (grp) return launch_pers<T, 4, false, 192, true>(xmap, a, m_tiles, st);                        \
         if (ks == 4) return launch_gemm<T, 4, 4, true>(xmap, a, m_tiles, st);                             \
         if (ks == 2) return launch_gemm<T, 4, 2, true>(xmap, a, m_tiles, st);                             \
@@ -1135,21 +1184,23 @@ int jq_mxfp4_gemm(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint
 int jq_mxfp4_moe_gemm(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx, const int32_t* expert_offsets,
                       const int32_t* tile_expert, const int32_t* tile_row0, const int32_t* num_tiles, int64_t max_tiles,
                       int tile_m, const uint32_t* const* codes_tab, const uint8_t* const* scales_tab, int64_t N, int64_t K,
-                      void* y_sorted, int64_t ldy, jq_stream_t stream) {
+                      const int32_t* order, const int32_t* inv, void* y, int64_t ldy, jq_stream_t stream) {
     using namespace jq;
     int rc = check_mxfp4_gemm(N, K);
     if (rc != JQ_OK) return rc;
     JQ_REQUIRE(tile_m == 128 || tile_m == 192, JQ_EINVAL, "tile_m must be 128 or 192");
     JQ_REQUIRE(expert_offsets && tile_expert && tile_row0 && num_tiles && codes_tab && scales_tab, JQ_EINVAL, "null pointer");
-    JQ_REQUIRE(max_tiles >= 0, JQ_EINVAL, "negative max_tiles");
+    JQ_REQUIRE((order != nullptr) == (inv != nullptr), JQ_EINVAL, "order and inv come together");
+    JQ_REQUIRE(max_tiles > 0 || (max_tiles == 0 && !order), JQ_EINVAL, "max_tiles must be positive");
     GroupedArgs g;
     g.tile_expert = tile_expert; g.tile_row0 = tile_row0; g.num_tiles = num_tiles; g.expert_offsets = expert_offsets;
     g.bits_tab = nullptr; g.codes_tab = codes_tab;
     g.scales_tab = g.biases_tab = reinterpret_cast<const void* const*>(scales_tab);
     g.max_tiles = max_tiles;
     g.tile_m = tile_m;
-    return qgemm_dispatch(x_sorted, act_dtype, max_rows, ldx, nullptr, nullptr, nullptr, act_dtype, N, K, 4, 64, y_sorted,
-                          act_dtype, ldy, &g, (cudaStream_t)stream, true);
+    g.order = order; g.inv = inv;
+    return qgemm_dispatch(x_sorted, act_dtype, max_rows, ldx, nullptr, nullptr, nullptr, act_dtype, N, K, 4, 64, y, act_dtype,
+                          ldy, &g, (cudaStream_t)stream, true);
 }
 
 int jq_mxfp4_moe_gate_up_swiglu(const void* x_sorted, int act_dtype, int64_t max_rows, int64_t ldx,

@@ -185,14 +185,16 @@ def expert_gemv(x: torch.Tensor, x_div: int, pair_expert: torch.Tensor, bank: MX
     return y
 
 
-def expert_gemm(x_sorted: torch.Tensor, sp, bank: MXFP4ExpertBank) -> torch.Tensor:
-    """The grouped product over expert-sorted rows (moe.SortedPairs)."""
+def expert_gemm(x_sorted: torch.Tensor, sp, bank: MXFP4ExpertBank, scatter: bool = False) -> torch.Tensor:
+    """The grouped product over expert-sorted rows (moe.SortedPairs); scatter=True stores the rows where their pairs stand,
+    and zeros for the pairs of no expert of the bank."""
     lib = _lib.load()
     y = x_sorted.new_empty((x_sorted.shape[0], bank.N))
     _lib.check(lib.jq_mxfp4_moe_gemm(x_sorted.data_ptr(), _lib.dtype_id(x_sorted.dtype), sp.n, x_sorted.stride(0),
                                      sp.offsets.data_ptr(), sp.tile_expert.data_ptr(), sp.tile_row0.data_ptr(),
                                      sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, bank.codes_tab.data_ptr(),
-                                     bank.scales_tab.data_ptr(), bank.N, bank.K, y.data_ptr(), bank.N,
+                                     bank.scales_tab.data_ptr(), bank.N, bank.K, sp.order.data_ptr() if scatter else None,
+                                     sp.inv.data_ptr() if scatter else None, y.data_ptr(), bank.N,
                                      _lib.stream_ptr(x_sorted.device)))
     return y
 
@@ -240,9 +242,4 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
             return expert_gemv(x2, x_div, rhs, bank)
         from . import moe
         sp = moe.SortedPairs(rhs, bank.E, tile_m=_lib.MOE_GEMM_TILE_M)
-        ys = expert_gemm(moe._gather_rows(x2, sp, x_div), sp, bank)
-        y = x.new_empty((R, bank.N))
-        # back to the order of the pairs; pairs without an expert of the bank have no row and get zeros
-        _lib.check(_lib.load().jq_moe_combine_shared(ys.data_ptr(), ys.stride(0), sp.inv.data_ptr(), None, R, 1, bank.N, None, 0,
-                                                     y.data_ptr(), bank.N, None, _lib.dtype_id(x.dtype), _lib.stream_ptr(dev)))
-        return y
+        return expert_gemm(moe._gather_rows(x2, sp, x_div), sp, bank, scatter=True)

@@ -444,5 +444,6 @@ def test_argument_checks_need_no_gpu():
     assert lib.jq_mxfp4_gather_gemv(16, L.JQ_BF16, 64, 1, 16, 1 << 17, 16, 16, 1, 0, 4, 64, 16, 4, None) == L.JQ_EUNSUPPORTED
     assert lib.jq_mxfp4_gemm4(None, None, 4, None, None, 4, 64, None, L.JQ_BF16, 4, None) == L.JQ_EINVAL
     assert lib.jq_mxfp4_gemm4(8, 16, 4, 16, 16, 4, 64, 16, L.JQ_BF16, 4, None) == L.JQ_EINVAL
-    assert lib.jq_mxfp4_moe_gemm(16, L.JQ_BF16, 4, 64, 16, 16, 16, 16, 1, 256, 16, 16, 4, 64, 16, 4, None) == L.JQ_EINVAL
+    assert lib.jq_mxfp4_moe_gemm(16, L.JQ_BF16, 4, 64, 16, 16, 16, 16, 1, 256, 16, 16, 4, 64, None, None, 16, 4, None) == L.JQ_EINVAL
+    assert lib.jq_mxfp4_moe_gemm(16, L.JQ_BF16, 4, 64, 16, 16, 16, 16, 1, 192, 16, 16, 4, 64, 16, None, 16, 4, None) == L.JQ_EINVAL
     assert lib.jq_moe_route_topk(16, L.JQ_F32, 8, 1, 8, 2, 2, None, 1, 1, 1, 1, 1.0, 16, 16, None) == L.JQ_EINVAL
