@@ -5,12 +5,16 @@
 //   idx = the k largest c of the groups that stay, descending;  w = s[idx] (/ (sum + 1e-20)) * scale
 //
 // Bound: T * E logits read once; at the sizes of a serving step it is latency, the k dependent selections of a warp.
-// One warp per token, a lane holds PER >= E / 32 of the row's keys in registers.  Which expert is taken hangs on
-// neighbouring scores, so c is compared in float64 (float32 scores put close neighbours on the wrong side about once in
-// 4096 tokens x 256 experts); where c grows with the logit alone -- no bias, and at most the best expert of a group
-// counts -- the order of the logits is the order of the scores and 32-bit keys do.  A key is the value's bits made
-// monotonic as an unsigned integer, so an arg-max over the warp is two redux steps per 32 bits instead of ten
-// shuffles; equal keys go to the lower expert.  A NaN logit counts as -inf, a score of zero; +inf takes the limit.
+// One warp per token, a lane holds PER >= E / 32 of the row's keys in registers: values made monotonic as unsigned
+// integers, so the arg-max of the warp is two redux steps; equal keys go to the lower expert.
+// Which expert is taken hangs on neighbouring scores: float32 scores put close neighbours on the wrong side about once in
+// 4096 tokens x 256 experts, and float64 ones for every expert cost 12 us for 61 tokens x 512.  So a token is selected on
+// float32 scores together with a bound of their error, and what the bound leaves open is settled in float64: the groups, if
+// two at the cut are closer than the bound, and the order of the chosen experts and of those within the bound of the last,
+// if there are neighbours among them that close.  The slowest token of a call is its time, so this path is kept short too
+// (the whole token again in float64: 22 us for 4096 x 256).  Where c grows with the logit alone (no bias, and at most the
+// best expert of a group counts) the order of the logits is the order of the scores, exactly.  A NaN logit counts as -inf, a
+// score of zero; +inf takes the limit.
 #include "jq_common.cuh"
 
 namespace jq {
@@ -28,6 +32,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     const uint32_t b = __float_as_uint(v);
     return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 __device__ __forceinline__ uint64_t order_key(double v) {
     v = v != v ? -(double)INFINITY : v + 0.0;
     const uint64_t b = (uint64_t)__double_as_longlong(v);
@@ -41,8 +46,46 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     return (uint64_t)hi << 32 | lo;
 }
 
-template <bool F64> struct RouteKey { using V = float; using K = uint32_t; };
-template <> struct RouteKey<true> { using V = double; using K = uint64_t; };
+// How the choice scores are held: the logits themselves (their order is the scores'), or float32 with a bound of the error.
+enum RouteMode { ROUTE_LOGIT, ROUTE_SCREEN };
+// How far the difference of two float32 choice scores may be off, in units u = 2^-23.  The fast exponential of -d is off by
+// 2 + 1.16 d units of its value.  A softmax score is at most top = 1 / sum: exponential 2 top (where d = 0), its argument and the
+// quotient 1.5 top; the sum, common to both scores, by the mean of 2 + 1.16 d over the terms, at most 11 for 1024 experts, and
+// ten additions by halves: 16 top for the difference.  23 top for two scores.  A sigmoid score is off by 1 from its
+// exponential (s (1 - s) (2 + 1.16 d) < 1), 2 from the quotient and 1 from the sum in it: 8 for two.  The sum of a group's
+// two largest is off by twice as much.  Adding the bias rounds each by half a unit of |c|, the group's sum once more: 4 of the
+// largest |c|.  46 top, 16 and 4, each taken about twice as large.
+__device__ __forceinline__ float choice_error(bool sigmoid, float top, float largest) {
+    return (sigmoid ? 0x1p-18f : 0x1p-16f * top) + 0x1p-20f * largest;
+}
+
+// sum by halves (E of 1024: ten additions deep), and the largest key with its place, the lower place on ties
+template <int PER> __device__ __forceinline__ float lane_sum(const float (&c)[PER]) {
+    float p[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) p[i] = c[i];
+#pragma unroll
+    for (int w = PER / 2; w > 0; w /= 2)
+#pragma unroll
+        for (int i = 0; i < w; ++i) p[i] += p[i + w];
+    return p[0];
+}
+template <int PER> __device__ __forceinline__ void lane_best(const uint32_t (&key)[PER], uint32_t& best, int& at) {
+    uint32_t k[PER];
+    int ix[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { k[i] = key[i]; ix[i] = i; }
+#pragma unroll
+    for (int w = PER / 2; w > 0; w /= 2)
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const bool left = k[2 * i] >= k[2 * i + 1];
+            k[i] = left ? k[2 * i] : k[2 * i + 1];
+            ix[i] = left ? ix[2 * i] : ix[2 * i + 1];
+        }
+    best = k[0];
+    at = ix[0];
+}
 
 struct RouteArgs {
     const void* logits;
@@ -51,6 +94,7 @@ struct RouteArgs {
     int32_t* idx;
     float* w;
     int T, E, k, sigmoid, groups, kept, top, renorm;
+    int per;                         // experts of a group
     float scale;
 };
 
@@ -61,167 +105,293 @@ template <typename LT> __device__ __forceinline__ float load_logit(const RouteAr
 // exp(l - mx) without inf - inf
 __device__ __forceinline__ double exp_below(float l, float mx) { return l == mx ? (mx == -INFINITY ? 0.0 : 1.0) : exp((double)l - (double)mx); }
 
-template <typename LT, int PER, bool F64>
-__global__ void __launch_bounds__(32 * ROUTE2_WARPS)
-route_groups_kernel(const RouteArgs a) {
-    using V = typename RouteKey<F64>::V;
-    using K = typename RouteKey<F64>::K;
-    extern __shared__ __align__(16) uint8_t route_smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t t = (int64_t)blockIdx.x * ROUTE2_WARPS + warp;
-    if (t >= a.T) return;                                  // no block-wide barrier below
-    const int E = a.E;
+// Which groups stay, as a bit per group, from the choice scores of the token in shared memory.  near: set (in every lane)
+// when a group at the cut is within `close` of another.
+template <typename V>
+__device__ __forceinline__ uint32_t kept_groups(const RouteArgs& a, const V* row, int lane, float close, bool& near) {
+    // L lanes per group (a power of two): two largest of the lane's share, then a butterfly over the L lanes
+    int L = 1;
+    while (2 * L * a.groups <= 32) L *= 2;
+    const int g = lane / L;
+    V best = -(V)INFINITY, second = -(V)INFINITY;
+    if (g < a.groups)
+        for (int j = lane % L; j < a.per; j += L) {
+            const V v = row[g * a.per + j];
+            second = v > best ? best : (v > second ? v : second);
+            best = v > best ? v : best;
+        }
+    for (int d = L / 2; d > 0; d >>= 1) {
+        const V b2 = __shfl_xor_sync(0xFFFFFFFFu, best, d), s2 = __shfl_xor_sync(0xFFFFFFFFu, second, d);
+        const V low = best < b2 ? best : b2, high = best < b2 ? b2 : best;
+        const V s = second > s2 ? second : s2;
+        best = high;
+        second = low > s ? low : s;
+    }
+    const V score = a.top == 2 ? best + second : best;
+    const auto mine = order_key(score);
+    int rank = 0;
+    bool touch = false;
+    for (int o = 0; o < a.groups; ++o) {
+        const auto other = __shfl_sync(0xFFFFFFFFu, mine, o * L);
+        const V value = __shfl_sync(0xFFFFFFFFu, score, o * L);
+        rank += (other > mine || (other == mine && o < g)) ? 1 : 0;
+        touch |= o != g && !(fabs(value - score) > (V)close);            // two infinities differ by NaN, which is near
+    }
+    near = __any_sync(0xFFFFFFFFu, g < a.groups && touch && (rank == a.kept - 1 || rank == a.kept));
+    const uint32_t in = __ballot_sync(0xFFFFFFFFu, g < a.groups && rank < a.kept);      // L equal bits per group
+    uint32_t keep = 0;
+    for (int o = 0; o < a.groups; ++o) keep |= ((in >> (o * L)) & 1u) << o;
+    return keep;
+}
 
-    float l[PER];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        l[i] = e < E ? load_logit<LT>(a, t, e) : -INFINITY;
-        mx = fmaxf(mx, l[i]);
+// Results of up to 32 selections from j0 on: lane j holds expert `mine`.  Returns the sum of their scores.
+template <typename LT>
+__device__ __forceinline__ double store_chosen(const RouteArgs& a, int64_t t, int lane, int j0, int n, int mine, float mx, double sum) {
+    double s = 0.0, chosen;
+    if (lane < n) {
+        const float lv = load_logit<LT>(a, t, mine);
+        s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
+        a.idx[t * a.k + j0 + lane] = mine;
     }
-    double sum = 0.0;                                      // of the softmax; unused with sigmoid scores
-    V c[PER];
-    if (!a.sigmoid) {
+    chosen = s;
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-        if constexpr (F64) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                c[i] = lane + 32 * i < E ? exp_below(l[i], mx) : 0.0;
-                sum += c[i];
-            }
-        } else {                                           // only the weights see the sum: float32 terms
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (l[i] != -INFINITY) part += l[i] == mx ? 1.f : expf(l[i] - mx);
-            sum = part;
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-        if (sum == 0.0) sum = 1.0;                         // a row of -inf: every score is zero
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        if constexpr (F64) {
-            c[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : c[i] / sum;
-            if (a.bias && e < E) c[i] += (double)a.bias[e];
-        } else {
-            c[i] = l[i];
-        }
-    }
-
-    uint32_t keep = 0xFFFFFFFFu;                           // bit per group
-    const int per = E / a.groups;
-    if (a.groups > 1) {
-        V* row = reinterpret_cast<V*>(route_smem) + (size_t)warp * E;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < E) row[lane + 32 * i] = c[i] != c[i] ? -(V)INFINITY : c[i];
-        __syncwarp();
-        // L lanes per group (a power of two): two largest of the lane's share, then a butterfly over the L lanes
-        int L = 1;
-        while (2 * L * a.groups <= 32) L *= 2;
-        const int g = lane / L;
-        V best = -(V)INFINITY, second = -(V)INFINITY;
-        if (g < a.groups)
-            for (int j = lane % L; j < per; j += L) {
-                const V v = row[g * per + j];
-                second = v > best ? best : (v > second ? v : second);
-                best = v > best ? v : best;
-            }
-        for (int d = L / 2; d > 0; d >>= 1) {
-            const V b2 = __shfl_xor_sync(0xFFFFFFFFu, best, d), s2 = __shfl_xor_sync(0xFFFFFFFFu, second, d);
-            const V low = best < b2 ? best : b2, high = best < b2 ? b2 : best;
-            const V s = second > s2 ? second : s2;
-            best = high;
-            second = low > s ? low : s;
-        }
-        const K mine = order_key(a.top == 2 ? best + second : best);
-        int rank = 0;
-        for (int o = 0; o < a.groups; ++o) {
-            const K other = __shfl_sync(0xFFFFFFFFu, mine, o * L);
-            rank += (other > mine || (other == mine && o < g)) ? 1 : 0;
-        }
-        const uint32_t in = __ballot_sync(0xFFFFFFFFu, g < a.groups && rank < a.kept);      // L equal bits per group
-        keep = 0;
-        for (int o = 0; o < a.groups; ++o) keep |= ((in >> (o * L)) & 1u) << o;
-    }
-
-    K key[PER];
-    K best = 0;
-    int bi = 0;                                            // register index of the lane's best; the lower expert on ties
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = e < E && (a.groups == 1 || (keep >> (e / per) & 1u)) ? order_key(c[i]) : (K)0;
-        if (key[i] > best) { best = key[i]; bi = i; }
-    }
-    double chosen = 0.0;                                   // sum of the chosen scores
-    for (int j0 = 0; j0 < a.k; j0 += 32) {
-        const int n = min(32, a.k - j0);
-        int mine = 0;
-        for (int j = 0; j < n; ++j) {
-            const K top = warp_max(best);
-            const int e = (int)redux_min(best == top ? (uint32_t)(lane + 32 * bi) : 0xFFFFFFFFu);
-            if (lane == j) mine = e;
-            if (lane == (e & 31)) {                        // the owner looks for its next one
-                best = 0;
-                const int gone = e >> 5;
-                bi = 0;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    if (i == gone) key[i] = 0;
-                    if (key[i] > best) { best = key[i]; bi = i; }
-                }
-            }
-            __syncwarp();
-        }
-        double s = 0.0;
-        if (lane < n) {
-            const float lv = load_logit<LT>(a, t, mine);
-            s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
-            a.idx[t * a.k + j0 + lane] = mine;
-        }
-        chosen += s;
-        if (a.k > 32 && lane < n) a.w[t * a.k + j0 + lane] = (float)s;        // scaled below, once the sum is known
-        if (a.k <= 32) {
-            double norm = a.scale;
-            if (a.renorm) {
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) chosen += __shfl_xor_sync(0xFFFFFFFFu, chosen, d);
-                norm = (double)a.scale / (chosen + 1e-20);
-            }
-            if (lane < n) a.w[t * a.k + lane] = (float)(s * norm);
-            return;
-        }
-    }
-    double norm = a.scale;
-    if (a.renorm) {
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) chosen += __shfl_xor_sync(0xFFFFFFFFu, chosen, d);
-        norm = (double)a.scale / (chosen + 1e-20);
-    }
-    for (int j = lane; j < a.k; j += 32) {                 // the lane's own stores of above
+    for (int d = 16; d > 0; d >>= 1) chosen += __shfl_xor_sync(0xFFFFFFFFu, chosen, d);
+    if (a.k <= 32) s *= a.renorm ? (double)a.scale / (chosen + 1e-20) : (double)a.scale;
+    if (lane < n) a.w[t * a.k + j0 + lane] = (float)s;     // of more than 32: scaled when the sum is known
+    return chosen;
+}
+__device__ __forceinline__ void scale_chosen(const RouteArgs& a, int64_t t, int lane, double chosen) {
+    if (a.k <= 32) return;
+    const double norm = a.renorm ? (double)a.scale / (chosen + 1e-20) : (double)a.scale;
+    for (int j = lane; j < a.k; j += 32) {                 // the lane's own stores
         float* p = a.w + t * a.k + j;
         *p = (float)((double)*p * norm);
     }
 }
 
-template <typename LT, int PER, bool F64>
+// Sum of the softmax, and the choice scores of a whole token, in float64; four exponentials at a time (a row of them unrolled is
+// so much code that fetching it takes longer than running it).
+template <typename LT>
+__device__ __noinline__ double exact_sum(const RouteArgs& a, int64_t t, int lane, float mx) {
+    double sum = 0.0;
+#pragma unroll 4
+    for (int e = lane; e < a.E; e += 32) sum += exp_below(load_logit<LT>(a, t, e), mx);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    return sum == 0.0 ? 1.0 : sum;                         // a row of -inf: every score is zero
+}
+template <typename LT>
+__device__ __forceinline__ double exact_choice(const RouteArgs& a, int64_t t, int e, float mx, double sum) {
+    const float lv = load_logit<LT>(a, t, e);
+    double c = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
+    if (a.bias) c += (double)a.bias[e];
+    return c != c ? -(double)INFINITY : c;
+}
+template <typename LT>
+__device__ __noinline__ void exact_row(const RouteArgs& a, int64_t t, int lane, double* row, float mx, double sum) {
+#pragma unroll 4
+    for (int e = lane; e < a.E; e += 32) row[e] = exact_choice<LT>(a, t, e, mx, sum);
+    __syncwarp();
+}
+
+// One token on 32-bit keys (row: E doubles of shared memory, or floats where the logits decide).  Returns false (the same in
+// every lane, nothing written) where more than 32 experts are too close to tell.
+template <typename LT, int PER, RouteMode MODE>
+__device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int lane, void* row, const float (&l)[PER], float mx) {
+    const int E = a.E;
+    float sum = 1.f;                                       // of the softmax
+    float c[PER];
+    // With renormalised weights the sum cancels and serves the screen alone; where it is in the weights (never read before the
+    // choice when the logits decide), the accurate exponential is used.
+    if (!a.sigmoid && (MODE == ROUTE_SCREEN || !a.renorm)) {
+        const float m = mx == -INFINITY ? 0.f : mx;        // exp(-inf) = 0 of masked experts, places past E and empty rows
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float d = mx == INFINITY ? (l[i] == INFINITY ? 0.f : -INFINITY) : l[i] - m;
+            c[i] = MODE == ROUTE_SCREEN ? __expf(d) : expf(d);
+        }
+        sum = lane_sum<PER>(c);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        if (sum == 0.f) sum = 1.f;                         // a row of -inf: every score is zero
+    }
+    float close = 0.f;
+    double sum64 = 0.0;                                    // computed when it is needed
+    if constexpr (MODE == ROUTE_LOGIT) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] = l[i];
+    } else {
+        float largest = 0.f;                               // |c| of the token; a NaN is passed over, it counts as -inf
+        const float inv = 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = lane + 32 * i;
+            c[i] = a.sigmoid ? __fdividef(1.f, 1.f + __expf(-l[i])) : c[i] * inv;
+            if (a.bias && e < E) c[i] += a.bias[e];
+            largest = fmaxf(largest, fabsf(c[i]));
+        }
+        close = choice_error(a.sigmoid, inv, __uint_as_float(redux_max(__float_as_uint(largest))));
+        if (!(close < INFINITY)) return false;             // an infinite bias
+    }
+    uint32_t keep = 0xFFFFFFFFu;
+    if (a.groups > 1) {
+        float* row32 = reinterpret_cast<float*>(row);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (lane + 32 * i < E) row32[lane + 32 * i] = c[i] != c[i] ? -INFINITY : c[i];
+        __syncwarp();
+        bool near;
+        keep = kept_groups<float>(a, row32, lane, close, near);
+        __syncwarp();                                      // the row is written again
+        if (MODE == ROUTE_SCREEN && near) {
+            if (!a.sigmoid) sum64 = exact_sum<LT>(a, t, lane, mx);
+            exact_row<LT>(a, t, lane, reinterpret_cast<double*>(row), mx, sum64);
+            keep = kept_groups<double>(a, reinterpret_cast<double*>(row), lane, 0.f, near);
+            __syncwarp();
+        }
+    }
+    uint32_t key[PER];
+    const float per_group = 1.f / (float)a.per;            // (e + 1/2) / per is never within 2^-12 of a whole number
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = e < E && (keep >> (int)(((float)e + 0.5f) * per_group) & 1u) ? order_key(c[i]) : 0u;
+    }
+    uint32_t best, before = 0;
+    int bi;                                                // register index of the lane's best
+    lane_best<PER>(key, best, bi);
+    double chosen = 0.0;
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+        int n = min(32, a.k - j0), mine = 0;
+        bool open = false;
+        for (int j = 0;; ++j) {
+            const uint32_t top = redux_max(best);
+            if (MODE == ROUTE_LOGIT && j == n) break;
+            if constexpr (MODE == ROUTE_SCREEN) {          // two infinities differ by NaN, which is close
+                const bool touch = j > 0 && top != 0 && !(key_value(before) - key_value(top) > close);
+                if (j >= n && !touch) break;               // the chosen ones and those within the bound of the last of them
+                if (j == 32) return false;
+                open |= touch;
+                before = top;
+            }
+            const int e = (int)redux_min(best == top ? (uint32_t)(lane + 32 * bi) : 0xFFFFFFFFu);
+            if (lane == j) mine = e;
+            if (lane == (e & 31)) {                        // the owner looks for its next one
+                const int gone = e >> 5;
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (i == gone) key[i] = 0;
+                lane_best<PER>(key, best, bi);
+            }
+            __syncwarp();
+            if constexpr (MODE == ROUTE_SCREEN)
+                if (j >= n) n = j + 1;
+        }
+        if constexpr (MODE == ROUTE_SCREEN) {
+            if (open) {                                    // k <= 32 here: order the n candidates by their exact scores
+                if (!a.sigmoid && sum64 == 0.0) sum64 = exact_sum<LT>(a, t, lane, mx);
+                const uint64_t k64 = lane < n ? order_key(exact_choice<LT>(a, t, mine, mx, sum64)) : 0ull;
+                int rank = 0;
+                for (int o = 0; o < n; ++o) {
+                    const uint64_t other = __shfl_sync(0xFFFFFFFFu, k64, o);
+                    const int oe = __shfl_sync(0xFFFFFFFFu, mine, o);
+                    rank += other > k64 || (other == k64 && oe < mine) ? 1 : 0;
+                }
+                int* place = reinterpret_cast<int*>(row);  // E >= n of them
+                if (lane < n) place[rank] = mine;
+                __syncwarp();
+                mine = lane < n ? place[lane] : 0;
+            }
+            n = min(32, a.k - j0);
+        }
+        if constexpr (MODE == ROUTE_SCREEN)                // the screen's sum is too rough for weights that hold it
+            if (!a.sigmoid && !a.renorm && sum64 == 0.0) sum64 = exact_sum<LT>(a, t, lane, mx);
+        chosen += store_chosen<LT>(a, t, lane, j0, n, mine, mx, sum64 != 0.0 ? sum64 : (double)sum);
+    }
+    scale_chosen(a, t, lane, chosen);
+    return true;
+}
+
+// A whole token in float64, in shared memory: more than 32 experts to choose, or too many too close to each other.
+template <typename LT>
+__device__ __noinline__ void route_token_exact(const RouteArgs& a, int64_t t, int lane, double* row, float mx) {
+    const double sum = a.sigmoid ? 1.0 : exact_sum<LT>(a, t, lane, mx);
+    exact_row<LT>(a, t, lane, row, mx, sum);
+    uint32_t keep = 0xFFFFFFFFu;
+    if (a.groups > 1) {
+        bool near;
+        keep = kept_groups<double>(a, row, lane, 0.f, near);
+        __syncwarp();
+    }
+    // keys take the scores' places; the lane's best is found by walking its share
+    uint64_t* key = reinterpret_cast<uint64_t*>(row);
+    uint64_t best = 0;
+    int at = 0;
+    for (int e = lane; e < a.E; e += 32) {
+        const uint64_t k = a.groups == 1 || (keep >> (e / a.per) & 1u) ? order_key(row[e]) : 0ull;
+        key[e] = k;
+        if (k > best) { best = k; at = e; }
+    }
+    double chosen = 0.0;
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+        const int n = min(32, a.k - j0);
+        int mine = 0;
+        for (int j = 0; j < n; ++j) {
+            const uint64_t top = warp_max(best);
+            const int e = (int)redux_min(best == top ? (uint32_t)at : 0xFFFFFFFFu);
+            if (lane == j) mine = e;
+            if (lane == (e & 31)) {
+                key[e] = 0;
+                best = 0;
+                for (int i = lane; i < a.E; i += 32)
+                    if (key[i] > best) { best = key[i]; at = i; }
+            }
+            __syncwarp();
+        }
+        chosen += store_chosen<LT>(a, t, lane, j0, n, mine, mx, sum);
+    }
+    scale_chosen(a, t, lane, chosen);
+}
+
+// SCREEN: the order of the logits does not decide
+template <typename LT, int PER, bool SCREEN>
+__global__ void __launch_bounds__(32 * ROUTE2_WARPS)
+route_groups_kernel(const RouteArgs a) {
+    extern __shared__ __align__(16) uint8_t route_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t = (int64_t)blockIdx.x * ROUTE2_WARPS + warp;
+    if (t >= a.T) return;                                  // no block-wide barrier below
+    float l[PER];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = lane + 32 * i;
+        l[i] = e < a.E ? load_logit<LT>(a, t, e) : -INFINITY;
+        mx = fmaxf(mx, l[i]);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+    if constexpr (SCREEN) {
+        double* row = reinterpret_cast<double*>(route_smem) + (size_t)warp * a.E;
+        if (a.k > 32 || !route_token<LT, PER, ROUTE_SCREEN>(a, t, lane, row, l, mx))
+            route_token_exact<LT>(a, t, lane, row, mx);
+    } else {
+        route_token<LT, PER, ROUTE_LOGIT>(a, t, lane, reinterpret_cast<float*>(route_smem) + (size_t)warp * a.E, l, mx);
+    }
+}
+
+template <typename LT, int PER, bool SCREEN>
 static int launch_route(const RouteArgs& a, cudaStream_t st) {
     const unsigned blocks = (unsigned)((a.T + ROUTE2_WARPS - 1) / ROUTE2_WARPS);
-    const size_t smem = a.groups > 1 ? (size_t)ROUTE2_WARPS * a.E * sizeof(typename RouteKey<F64>::V) : 0;
+    const size_t smem = SCREEN || a.groups > 1 ? (size_t)ROUTE2_WARPS * a.E * (SCREEN ? sizeof(double) : sizeof(float)) : 0;
     static_assert(ROUTE2_WARPS * ROUTE2_MAX_E * sizeof(double) <= 48 * 1024, "no opt-in shared memory");
-    route_groups_kernel<LT, PER, F64><<<blocks, 32 * ROUTE2_WARPS, smem, st>>>(a);
+    route_groups_kernel<LT, PER, SCREEN><<<blocks, 32 * ROUTE2_WARPS, smem, st>>>(a);
     return check_launch("moe_route_topk");
 }
 
 template <typename LT>
-static int launch_route_e(const RouteArgs& a, bool f64, cudaStream_t st) {
-#define JQ_ROUTE_PER(P) return f64 ? launch_route<LT, P, true>(a, st) : launch_route<LT, P, false>(a, st)
+static int launch_route_e(const RouteArgs& a, bool screen, cudaStream_t st) {
+#define JQ_ROUTE_PER(P) return screen ? launch_route<LT, P, true>(a, st) : launch_route<LT, P, false>(a, st)
     if (a.E <= 64) JQ_ROUTE_PER(2);
     if (a.E <= 128) JQ_ROUTE_PER(4);
     if (a.E <= 256) JQ_ROUTE_PER(8);
@@ -256,8 +426,9 @@ extern "C" int jq_moe_route_topk(const void* logits, int logits_dtype, int64_t l
     a.T = (int)T; a.E = num_experts; a.k = k; a.sigmoid = score == JQ_SCORE_SIGMOID;
     // all groups kept is no grouping
     a.groups = groups_kept == groups ? 1 : groups;
+    a.per = num_experts / a.groups;
     a.kept = groups_kept; a.top = group_top; a.renorm = renorm; a.scale = scale;
-    const bool f64 = bias != nullptr || (a.groups > 1 && group_top == 2);
-    JQ_DISPATCH_DTYPE(logits_dtype, LT, return launch_route_e<LT>(a, f64, (cudaStream_t)stream));
+    const bool screen = bias != nullptr || (a.groups > 1 && group_top == 2);
+    JQ_DISPATCH_DTYPE(logits_dtype, LT, return launch_route_e<LT>(a, screen, (cudaStream_t)stream));
     return JQ_OK;
 }
