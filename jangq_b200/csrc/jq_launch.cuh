@@ -1,0 +1,30 @@
+// Launches that may be scheduled while their predecessor on the stream still runs (programmatic stream serialization).
+#pragma once
+
+#include "jq_common.cuh"
+
+namespace jq {
+
+// First statement of such a kernel, in every thread: the successor may be scheduled from here on, and no memory is touched
+// before all earlier work of the stream is complete and visible.
+__device__ __forceinline__ void overlap_enter() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace jq

@@ -8,6 +8,7 @@
 // takes two shuffles.  The product with 2^-e is exact in f32, so the conversion instruction's rounding is the only one.
 #include <algorithm>
 
+#include "jq_launch.cuh"
 #include "jq_mxfp4.cuh"
 
 namespace jq {
@@ -37,17 +38,24 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
     return r;
 }
 
-// words: multiple of 4, so the four lanes of a block are in range together; the grid's stride is a multiple of 32
-template <typename T>
+// A thread takes U words, a CTA's width apart.  words is a multiple of 4 and the steps are multiples of 32, so the four lanes
+// of a block are in range together.
+template <typename T, int U>
 __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const T* __restrict__ w, int64_t words, uint32_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += step) {
-        float v[8];
-        load8(w + i * 8, v);
+    overlap_enter();
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (i0 + u * 256 < words) load8(w + (i0 + u * 256) * 8, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t i = i0 + u * 256;
+        if (i >= words) break;
         uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[u][j]) & 0x7FFFFFFFu);
         const uint32_t four = 0xFu << (threadIdx.x & 28);
         m = max(m, __shfl_xor_sync(four, m, 1));
         m = max(m, __shfl_xor_sync(four, m, 2));
@@ -55,18 +63,29 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const T* __restrict
         const uint32_t byte = ex == 255u ? 255u : (ex > 2u ? ex - 2u : 0u);
         const float inv = __uint_as_float((254u - min(byte, 253u)) << 23);     // 2^-e; 2^127 at byte 0
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
-        codes[i] = byte == 255u ? 0u : e2m1x8(v);
+        for (int j = 0; j < 8; ++j) v[u][j] *= inv;
+        codes[i] = byte == 255u ? 0u : e2m1x8(v[u]);
         if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)byte;
     }
 }
 
-template <typename T>
+template <typename T, int U>
 __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                                int64_t words, T* __restrict__ out) {
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += step) {
-        const uint32_t w = codes[i], b = scales[i >> 2];
+    overlap_enter();
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+    uint32_t ws[U], bs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (i0 + u * 256 < words) {
+            ws[u] = codes[i0 + u * 256];
+            bs[u] = scales[(i0 + u * 256) >> 2];
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t i = i0 + u * 256;
+        if (i >= words) break;
+        const uint32_t w = ws[u], b = bs[u];
         // 2^(b - 127) as f32: byte 0 is a subnormal, 255 not a number
         const float s = __uint_as_float(b == 0u ? 0x00400000u : (b == 255u ? 0x7FC00000u : b << 23));
         float v[8];
@@ -96,7 +115,12 @@ int check_mxfp4_shape(int64_t rows, int64_t K) {
     return JQ_OK;
 }
 
-static unsigned stream_grid(int64_t words) { return (unsigned)std::min<int64_t>((words + 255) / 256, (int64_t)sm_count() * 16); }
+// Words per thread: four where that still leaves every SM a full set of threads, one below.
+static bool four_words(int64_t words) { return words >= (int64_t)sm_count() * 2048 * 4; }
+static int check_words(int64_t words) {
+    JQ_REQUIRE(words / 256 < (1ll << 31) - 1, JQ_EUNSUPPORTED, "too many elements for one launch");
+    return JQ_OK;
+}
 
 }  // namespace jq
 
@@ -111,9 +135,13 @@ int jq_mxfp4_quantize(const void* w, int w_dtype, int64_t rows, int64_t K, uint3
     JQ_REQUIRE(w && codes && scales, JQ_EINVAL, "null pointer");
     JQ_REQUIRE(aligned(w, 16) && aligned(codes, 4), JQ_EINVAL, "w must be 16-byte aligned, codes 4-byte");
     const int64_t words = rows * (K / 8);
-    JQ_DISPATCH_DTYPE(w_dtype, T, mxfp4_quantize_kernel<T><<<stream_grid(words), 256, 0, (cudaStream_t)stream>>>(
-                                     (const T*)w, words, codes, scales));
-    return check_launch("mxfp4_quantize");
+    rc = check_words(words);
+    if (rc != JQ_OK) return rc;
+    const bool four = four_words(words);
+    const dim3 grid((unsigned)((words + (four ? 1023 : 255)) / (four ? 1024 : 256)));
+    JQ_DISPATCH_DTYPE(w_dtype, T, JQ_CUDA_OK(launch_overlapped(four ? mxfp4_quantize_kernel<T, 4> : mxfp4_quantize_kernel<T, 1>, grid, 256,
+                                                               0, (cudaStream_t)stream, (const T*)w, words, codes, scales)))
+    return JQ_OK;
 }
 
 int jq_mxfp4_dequantize(const uint32_t* codes, const uint8_t* scales, int64_t rows, int64_t K, void* out, int out_dtype,
@@ -126,9 +154,13 @@ int jq_mxfp4_dequantize(const uint32_t* codes, const uint8_t* scales, int64_t ro
     JQ_REQUIRE(codes && scales && out, JQ_EINVAL, "null pointer");
     JQ_REQUIRE(aligned(out, 16) && aligned(codes, 4), JQ_EINVAL, "out must be 16-byte aligned, codes 4-byte");
     const int64_t words = rows * (K / 8);
-    JQ_DISPATCH_DTYPE(out_dtype, T, mxfp4_dequantize_kernel<T><<<stream_grid(words), 256, 0, (cudaStream_t)stream>>>(
-                                       codes, scales, words, (T*)out));
-    return check_launch("mxfp4_dequantize");
+    rc = check_words(words);
+    if (rc != JQ_OK) return rc;
+    const bool four = four_words(words);
+    const dim3 grid((unsigned)((words + (four ? 1023 : 255)) / (four ? 1024 : 256)));
+    JQ_DISPATCH_DTYPE(out_dtype, T, JQ_CUDA_OK(launch_overlapped(four ? mxfp4_dequantize_kernel<T, 4> : mxfp4_dequantize_kernel<T, 1>, grid,
+                                                                 256, 0, (cudaStream_t)stream, codes, scales, words, (T*)out)))
+    return JQ_OK;
 }
 
 }  // extern "C"

@@ -10,6 +10,7 @@
 // The weight is exact in bf16; in f16 it is rounded once (scales below 2^-23 or above 2^13).
 #include <algorithm>
 
+#include "jq_launch.cuh"
 #include "jq_mxfp4.cuh"
 
 namespace jq {
@@ -54,6 +55,7 @@ __global__ void __launch_bounds__(32 * MXV_WARPS)
 mxfp4_gemv_kernel(const MxGemvArgs a) {
     using A = Act<AT>;
     __shared__ float part[MXV_WARPS][NT * 8][16 + 1];
+    overlap_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     const int64_t crow_bytes = a.nblk * 16;
@@ -176,9 +178,9 @@ int jq_mxfp4_gemv(const void* x, int x_dtype, int64_t M, int64_t ldx, const uint
     const dim3 grid((unsigned)((N + 15) / 16));
     cudaStream_t st = (cudaStream_t)stream;
     JQ_DISPATCH_DTYPE16(x_dtype, AT,
-        if (M <= 8) mxfp4_gemv_kernel<AT, 1, false><<<grid, 32 * MXV_WARPS, 0, st>>>(a);
-        else mxfp4_gemv_kernel<AT, 2, false><<<grid, 32 * MXV_WARPS, 0, st>>>(a));
-    return check_launch("mxfp4_gemv");
+        JQ_CUDA_OK(launch_overlapped(M <= 8 ? mxfp4_gemv_kernel<AT, 1, false> : mxfp4_gemv_kernel<AT, 2, false>, grid,
+                                     32 * MXV_WARPS, 0, st, a)))
+    return JQ_OK;
 }
 
 int jq_mxfp4_gather_gemv(const void* x, int x_dtype, int64_t ldx, int x_div, const int32_t* pair_expert, int64_t P,
@@ -197,8 +199,8 @@ int jq_mxfp4_gather_gemv(const void* x, int x_dtype, int64_t ldx, int x_div, con
     a.even = a.nblk % 2 == 0;
     const dim3 grid((unsigned)((N + 15) / 16), (unsigned)P);
     JQ_DISPATCH_DTYPE16(x_dtype, AT,
-        mxfp4_gemv_kernel<AT, 1, true><<<grid, 32 * MXV_WARPS, 0, (cudaStream_t)stream>>>(a));
-    return check_launch("mxfp4_gather_gemv");
+        JQ_CUDA_OK(launch_overlapped(mxfp4_gemv_kernel<AT, 1, true>, grid, 32 * MXV_WARPS, 0, (cudaStream_t)stream, a)))
+    return JQ_OK;
 }
 
 }  // extern "C"

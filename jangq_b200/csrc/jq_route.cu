@@ -15,7 +15,7 @@
 // (the whole token again in float64: 22 us for 4096 x 256).  Where c grows with the logit alone (no bias, and at most the
 // best expert of a group counts) the order of the logits is the order of the scores, exactly.  A NaN logit counts as -inf, a
 // score of zero; +inf takes the limit.
-#include "jq_common.cuh"
+#include "jq_launch.cuh"
 
 namespace jq {
 
@@ -358,6 +358,7 @@ template <typename LT, int PER, bool SCREEN>
 __global__ void __launch_bounds__(32 * ROUTE2_WARPS)
 route_groups_kernel(const RouteArgs a) {
     extern __shared__ __align__(16) uint8_t route_smem[];
+    overlap_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t = (int64_t)blockIdx.x * ROUTE2_WARPS + warp;
     if (t >= a.T) return;                                  // no block-wide barrier below
@@ -385,8 +386,8 @@ static int launch_route(const RouteArgs& a, cudaStream_t st) {
     const unsigned blocks = (unsigned)((a.T + ROUTE2_WARPS - 1) / ROUTE2_WARPS);
     const size_t smem = SCREEN || a.groups > 1 ? (size_t)ROUTE2_WARPS * a.E * (SCREEN ? sizeof(double) : sizeof(float)) : 0;
     static_assert(ROUTE2_WARPS * ROUTE2_MAX_E * sizeof(double) <= 48 * 1024, "no opt-in shared memory");
-    route_groups_kernel<LT, PER, SCREEN><<<blocks, 32 * ROUTE2_WARPS, smem, st>>>(a);
-    return check_launch("moe_route_topk");
+    JQ_CUDA_OK(launch_overlapped(route_groups_kernel<LT, PER, SCREEN>, dim3(blocks), 32 * ROUTE2_WARPS, smem, st, a));
+    return JQ_OK;
 }
 
 template <typename LT>
