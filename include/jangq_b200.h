@@ -513,12 +513,16 @@ int jq_mxfp4_quantize(const void* w, int w_dtype, int64_t rows, int64_t K, uint3
 int jq_mxfp4_dequantize(const uint32_t* codes, const uint8_t* scales, int64_t rows, int64_t K, void* out, int out_dtype,
                         jq_stream_t stream);
 
-/* y[M, N] = x[M, K] . deq(w)[N, K]^T, x and y of one 16-bit type, f32 sums.  The weight enters in x's type: exact in bf16,
- * rounded once in f16 (scales below 2^-23, and overflow to infinity above 2^13).  x 16-byte aligned with ldx % 8 == 0,
- * codes 16-byte, scales 2-byte aligned.
- *   jq_mxfp4_gemv: M <= 16, any K % 32 == 0;   jq_mxfp4_gemm: any M, K % 64 == 0 (tensor cores).
+/* y[M, N] = x[M, K] . deq(w)[N, K]^T, x and y of one 16-bit type, f32 sums.  In the tensor-core forms the weight enters in
+ * x's type: exact in bf16, rounded once in f16 (scales below 2^-23, and overflow to infinity above 2^13).  x 16-byte
+ * aligned with ldx % 8 == 0, codes 16-byte, scales 4-byte aligned.
+ *   jq_mxfp4_gemm: any M, K % 64 == 0 (tensor cores)
+ *   jq_mxfp4_gemv: M <= 16, K % 32 == 0 up to 36864.  Its products are of f16 pairs in any case: bf16 activations are
+ *   scaled per block of 32 by a power of two, and those below 2^-29 of the largest of their block rounded (by less than
+ *   2^-39 of it); the weight's scale multiplies the block's f32 sum, so every weight is exact here.
  * jq_mxfp4_gather_gemv: y[p] = x[p / x_div] . deq(w[pair_expert[p] - expert_base])^T for the pairs of routed experts; codes
- *   [num_experts, N, K/8] and scales [num_experts, N, K/32] are stacked; pairs of other experts get rows of zeros.
+ *   [num_experts, N, K/8] and scales [num_experts, N, K/32] are stacked; pairs of other experts get rows of zeros; K and
+ *   arithmetic as in jq_mxfp4_gemv.
  * jq_mxfp4_moe_gemm, jq_mxfp4_moe_gate_up_swiglu: jq_moe_gemm_tiled and jq_moe_gate_up_swiglu over MXFP4 experts (tile
  *   lists of 128 or 192 rows, pointer tables to codes and scales, which must be 16- and 2-byte aligned).  With order and
  *   inv of jq_moe_sort (both or neither) jq_mxfp4_moe_gemm stores its rows where the pairs stand, y[order[r]], and zeroes

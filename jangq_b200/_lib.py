@@ -25,6 +25,7 @@ JQ_GATHER_FEW_LOCAL = 2
 JQ_SCORE_SOFTMAX, JQ_SCORE_SIGMOID = 0, 1
 QGEMV_MAX_M = 16
 QGEMV_MAX_BATCH = 8
+MXFP4_GEMV_MAX_K = 36864
 MOE_TILE_M = 128
 MOE_GEMM_TILE_M = 192   # rows per tile of the grouped GEMMs (jq_moe_gemm_tiled, jq_moe_gate_up_swiglu)
 

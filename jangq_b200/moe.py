@@ -437,7 +437,7 @@ def _moe_layer_mxfp4(x, idx, w, gate, up, down, swiglu_limit, shared, expert_bas
     wf = w.reshape(-1).float().contiguous()
     dt, st = _lib.dtype_id(x.dtype), _lib.stream_ptr(dev)
     with _lib.on_device(dev):
-        use_sorted = P >= SORT_THRESHOLD if few_token_path is None else not few_token_path
+        use_sorted = gate.use_gemm(P) or down.use_gemm(P) if few_token_path is None else not few_token_path
         h = torch.empty((P, I), dtype=x.dtype, device=dev)
         if use_sorted and gate.gemm_ok and down.gemm_ok:
             sp = SortedPairs(idx32, gate.E, expert_base, tile_m=_lib.MOE_GEMM_TILE_M)

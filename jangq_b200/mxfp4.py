@@ -17,6 +17,10 @@ from ._lib import JangqError
 
 BLOCK = 32
 SORT_THRESHOLD = 64      # pairs; as gather_qmm
+# Rows that the mat-vec takes in one launch (their activations in shared memory: rows * K up to MXFP4_GEMV_MAX_K).  Beyond,
+# every weight is read again, and the tensor-core GEMM is faster: 8 rows of 14336x4096 17 us here, 23 there; 16 rows 57 and 23;
+# 2 rows of 4096x14336 16 and 21, 4 rows 30 and 21.
+MATVEC_ROWS = 8
 
 
 # A small product is a few microseconds of kernel, so the checks below take the short way where there is one: no slices and
@@ -97,8 +101,9 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
                  dtype: torch.dtype | None = None) -> torch.Tensor:
     """y[.., N] = x[.., K] . deq(w, scales)[N, K]^T with float32 sums.
 
-    x bfloat16 or float16: up to 16 rows run the mat-vec kernel, more the tensor-core GEMM; the output has x's type, and
-    the weight enters in it (exact in bfloat16; in float16 rounded once, and beyond 65504 infinite).
+    x bfloat16 or float16: few rows run the mat-vec kernel, more the tensor-core GEMM; the output has x's type.  In
+    the GEMM the weight enters in it (exact in bfloat16; in float16 rounded once, and beyond 65504 infinite); the mat-vec
+    rounds bfloat16 activations below 2^-29 of the largest of their block of 32, by less than 2^-39 of it.
     x int32 codes [.., K/8] with x_scales uint8 [.., K/32] (mxfp4_quantize of the activations): both operands go to the
     tensor cores in 4 bits; the output type is `dtype` (bfloat16 by default)."""
     dev = _lib.require_cuda(x, w, scales, x_scales)
@@ -129,9 +134,7 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
     dt, xp, yp, wp, sp = _lib.dtype_id(x.dtype), x2.data_ptr(), y.data_ptr(), w.data_ptr(), scales.data_ptr()
     with _lib.on_device(dev):
         st = _lib.stream_ptr(dev)
-        if M <= _lib.QGEMV_MAX_M:
-            _lib.check(lib.jq_mxfp4_gemv(xp, dt, M, ld, wp, sp, N, K, yp, N, st))
-        elif K % 64 == 0:
+        if K % 64 == 0 and (M > MATVEC_ROWS or M * K > _lib.MXFP4_GEMV_MAX_K):
             _lib.check(lib.jq_mxfp4_gemm(xp, dt, M, ld, wp, sp, N, K, yp, N, st))
         else:
             # an odd number of blocks is the mat-vec's, 16 rows at a time
@@ -167,6 +170,10 @@ class MXFP4ExpertBank:
     def gemm_ok(self) -> bool:
         """Shapes the tensor-core grouped product takes."""
         return self.K % 64 == 0
+
+    def use_gemm(self, pairs: int) -> bool:
+        """The grouped product, not a mat-vec per pair: many pairs, or rows too long for the mat-vec."""
+        return self.gemm_ok and (pairs >= SORT_THRESHOLD or self.K > _lib.MXFP4_GEMV_MAX_K)
 
 
 def expert_gemv(x: torch.Tensor, x_div: int, pair_expert: torch.Tensor, bank: MXFP4ExpertBank, expert_base: int = 0) -> torch.Tensor:
@@ -238,7 +245,7 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
         return x.new_empty((0, bank.N))
     x2 = rows_ok(x2)
     with _lib.on_device(dev):
-        if R < SORT_THRESHOLD or not bank.gemm_ok:
+        if not bank.use_gemm(R):
             return expert_gemv(x2, x_div, rhs, bank)
         from . import moe
         sp = moe.SortedPairs(rhs, bank.E, tile_m=_lib.MOE_GEMM_TILE_M)

@@ -111,11 +111,53 @@ def test_round_trip_of_representable_numbers():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 16, 64), (1, 200, 96), (1, 4096, 2048), (2, 33, 288), (3, 129, 2080), (5, 64, 4096),
-                                   (8, 1000, 320), (9, 15, 544), (16, 257, 2112), (1, 48, 14336), (16, 40, 8224)])
+                                   (8, 1000, 320), (9, 15, 544), (16, 257, 2112), (1, 48, 14336), (16, 40, 8224), (7, 24, 12320), (1, 20, 36864),
+                                   (2, 20, 36864), (1, 9, 40960)])
 def test_matvec(M, N, K, dtype):
     wq, s, v = _packed(M + N + K, (N, K))
     x = _rand(K, (M, K), dtype)
     _close(jq.mxfp4_matmul(x, wq, s), _np(x), v, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 20011, 4128), (3, 10007, 4128), (8, 9999, 2112), (2, 40003, 2112)])
+def test_matvec_over_many_tiles(M, N, K):
+    """More row tiles per SM than the kernel puts aside before it adds them."""
+    wq, s = jq.mxfp4_quantize(_rand(N, (N, K), "bf16", 0.02))
+    x = _rand(K, (M, K), "bf16")
+    w = jq.mxfp4_dequantize(wq, s, torch.float32).double()
+    ref, mag = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    y = jq.mxfp4_matmul(x, wq, s)
+    tol = 2.0 ** -8 * ref.abs() + (K / 16 + 32) * 2.0 ** -23 * mag
+    assert bool(((y.double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 2, 5])
+def test_matvec_activations_of_very_different_size(M):
+    """bf16 activations are scaled per block of 32, the largest to [2^14, 2^15), and rounded to f16, whose smallest step is 2^-24:
+    an activation is off by at most 2^-25 of that scale, 2^-39 of the largest of its block.  Other blocks are not touched."""
+    N, K = 64, 256
+    wq, s, v = _packed(31, (N, K))
+    x = _rand(32, (M, K), "bf16")
+    x[:, 40] = 2.0 ** 100
+    words = wq.clone()
+    words[:, 5] = 0                                        # weights 40 .. 47 are zero: only the small activations count
+    vz = v.copy()
+    vz[:, 40:48] = 0
+    x[:, 32:64] = torch.where(torch.arange(32, device="cuda") == 8, x[:, 32:64], x[:, 32:64] * 2.0 ** 72)
+    xn = _np(x)
+    for cols in (slice(0, 32), slice(32, 64)):
+        one = torch.zeros_like(x)
+        one[:, cols] = x[:, cols]
+        one[:, 40] = x[:, 40]
+        xo = _np(one)
+        y = jq.mxfp4_matmul(one, words, s)
+        ref, mag = xo @ vz.T, np.abs(xo) @ np.abs(vz).T
+        blocks = np.abs(xo).reshape(M, -1, 32).max(-1)
+        rounded = 2.0 ** -39 * (blocks[:, :, None] * np.abs(vz).reshape(N, -1, 32).sum(-1).T[None]).sum(1) if cols.start == 32 else 0.0
+        assert np.all(np.abs(_np(y) - ref) <= 2.0 ** -8 * np.abs(ref) + (K / 16 + 32) * 2.0 ** -23 * mag + rounded)
+    assert np.isfinite(xn).all()
 
 
 @pytest.mark.gpu
@@ -158,9 +200,9 @@ def test_row_and_column_of_a_product_are_their_own(M, K):
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 16, 64])
 def test_scales_over_the_whole_range(M):
-    """Bytes from 0 to 254: single products, so nothing is lost in a sum; and a NaN block spoils its own row only.  With
-    16-bit activations the weight enters in their type, so a weight above its largest number is infinite -- 4 * 2^126 at
-    byte 253 is 2^128, bf16 ends below it -- and the other, zero, activations make such a row NaN (0 * inf)."""
+    """Bytes from 0 to 254: single products, so nothing is lost in a sum; and a NaN block spoils its own row only.  In the
+    tensor-core GEMM (here 16 and 64 rows) the weight enters in the activations' type, so a weight above its largest number is infinite
+    -- 4 * 2^126 at byte 253 is 2^128, bf16 ends below it -- and the other, zero, activations make such a row NaN (0 * inf)."""
     K, N = 256, 255
     code = np.random.default_rng(3).integers(0, 16, (N, K)).astype(np.uint8)
     byte = np.repeat(np.arange(255, dtype=np.uint8)[:, None], K // 32, 1)
@@ -175,6 +217,10 @@ def test_scales_over_the_whole_range(M):
     def want(dtype, spoiled=None):
         w = torch.from_numpy(v).to(torch.float32).to(dtype)
         ref = w[:, torch.from_numpy(hot)].t().clone()
+        if M <= 8:                                         # the mat-vec scales the sums: every weight is exact
+            if spoiled is not None:
+                ref[:, spoiled] = float("nan")
+            return ref
         ref[:, w.isinf().any(1)] = float("nan")
         # every weight but the hot one meets a zero: a row whose only infinite weight is the hot one stays infinite
         for m, k in enumerate(hot):
@@ -275,6 +321,11 @@ def test_gather_with_experts_elsewhere_and_all_on_one(pairs):
     x = _rand(2, (pairs, K), "bf16")
     idx = torch.from_numpy(np.random.default_rng(3).integers(-2, E + 2, pairs)).int().cuda()
     _experts_close(jq.mxfp4_gather_matmul(x, wq, s, rhs_indices=idx), x, idx, v, 1)
+    bad = x.clone()
+    bad[:, 3] = float("nan")                               # not even the rows of pairs without an expert take it over
+    y = jq.mxfp4_gather_matmul(bad, wq, s, rhs_indices=idx)
+    away = (idx < 0) | (idx >= E)
+    assert not bool(y[away].any()) and bool(y[~away].isnan().all())
     for e in (0, 5, -1, E):
         _experts_close(jq.mxfp4_gather_matmul(x, wq, s, rhs_indices=torch.full_like(idx, e)), x, torch.full_like(idx, e), v, 1)
     assert jq.mxfp4_gather_matmul(x[:0], wq, s, rhs_indices=idx[:0]).shape == (0, N)
@@ -405,6 +456,7 @@ def test_refusals():
              lambda: jq.mxfp4_dequantize(wq[:, :0], s[:, :0]),
              lambda: jq.mxfp4_matmul(x[:, :96], wq, s), lambda: jq.mxfp4_matmul(x.float(), wq, s), lambda: jq.mxfp4_matmul(x, wq[None], s[None]),
              lambda: jq.mxfp4_matmul(x, wq, s, dtype=torch.float32), lambda: jq.mxfp4_matmul(x.cpu(), wq, s),
+             lambda: jq.mxfp4_matmul(z((2, 36896), torch.bfloat16), z((4, 4612), torch.int32), z((4, 1153), torch.uint8)),
              lambda: jq.mxfp4_matmul(wq, wq, s), lambda: jq.mxfp4_matmul(wq[:, :12], wq, s, x_scales=s[:, :3]),
              lambda: jq.mxfp4_matmul(wq, wq, s, x_scales=s, dtype=torch.float64), lambda: jq.mxfp4_matmul(x, wq, s, x_scales=s),
              lambda: jq.MXFP4ExpertBank(wq, s), lambda: jq.MXFP4ExpertBank(bank.weight[:0], bank.scales[:0]),
