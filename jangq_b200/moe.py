@@ -20,7 +20,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import JangqError
-from .mxfp4 import MXFP4ExpertBank, expert_gemm, expert_gemv, rows_ok
+from .mxfp4 import MXFP4ExpertBank, expert_gemm, expert_gemv, expert_ids, rows_ok
 
 SORT_THRESHOLD = 64      # pairs; dsv41/model.py:1206 (n * topk >= 64), mlx-lm SwitchGLU indices.size >= 64
 
@@ -420,8 +420,8 @@ def _moe_layer_mxfp4(x, idx, w, gate, up, down, swiglu_limit, shared, expert_bas
     """moe_layer over MXFP4 experts: the same two paths and the same order of operations."""
     lib = _lib.load()
     dev = _lib.require_cuda(x, idx, w, gate.weight, up.weight, down.weight)
-    if x.dim() != 2 or idx.dim() != 2 or idx.shape[0] != x.shape[0] or w.shape != idx.shape:
-        raise JangqError(_lib.JQ_EINVAL, f"moe_layer: x [T, H], idx and w [T, k], got {tuple(x.shape)}, {tuple(idx.shape)}, "
+    if x.dim() != 2 or idx.dim() != 2 or idx.shape[0] != x.shape[0] or idx.shape[1] < 1 or w.shape != idx.shape:
+        raise JangqError(_lib.JQ_EINVAL, f"moe_layer: x [T, H], idx and w [T, k >= 1], got {tuple(x.shape)}, {tuple(idx.shape)}, "
                                          f"{tuple(w.shape)}")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise JangqError(_lib.JQ_EINVAL, f"activations must be bfloat16 or float16, got {x.dtype}")
@@ -433,7 +433,7 @@ def _moe_layer_mxfp4(x, idx, w, gate, up, down, swiglu_limit, shared, expert_bas
     if T == 0:
         return torch.empty((0, down.N), dtype=torch.float32 if out_f32 else x.dtype, device=dev)
     x = rows_ok(x)
-    idx32 = idx.reshape(-1).to(torch.int32).contiguous()
+    idx32 = expert_ids(idx, expert_base, gate.E).reshape(-1)
     wf = w.reshape(-1).float().contiguous()
     dt, st = _lib.dtype_id(x.dtype), _lib.stream_ptr(dev)
     with _lib.on_device(dev):

@@ -172,8 +172,20 @@ class MXFP4ExpertBank:
         return self.K % 64 == 0
 
     def use_gemm(self, pairs: int) -> bool:
-        """The grouped product, not a mat-vec per pair: many pairs, or rows too long for the mat-vec."""
-        return self.gemm_ok and (pairs >= SORT_THRESHOLD or self.K > _lib.MXFP4_GEMV_MAX_K)
+        """The grouped product, not a mat-vec per pair: many pairs, or rows too long for the mat-vec (and no more experts
+        than the sort in front of it takes)."""
+        return self.gemm_ok and self.E <= 4096 and (pairs >= SORT_THRESHOLD or self.K > _lib.MXFP4_GEMV_MAX_K)
+
+
+def expert_ids(idx: torch.Tensor, base: int, experts: int) -> torch.Tensor:
+    """Contiguous int32 expert ids of the pairs; ids beyond 32 bits stay outside [base, base + experts)."""
+    if idx.dtype is torch.int32:
+        return idx if idx.is_contiguous() else idx.contiguous()
+    if idx.dtype is torch.int64:
+        idx = idx.clamp(base - 1, base + experts)
+    elif idx.is_floating_point() or idx.is_complex() or idx.dtype is torch.bool:
+        raise JangqError(_lib.JQ_EINVAL, f"expert indices must be integers, got {idx.dtype}")
+    return idx.to(torch.int32).contiguous()
 
 
 def expert_gemv(x: torch.Tensor, x_div: int, pair_expert: torch.Tensor, bank: MXFP4ExpertBank, expert_base: int = 0) -> torch.Tensor:
@@ -227,14 +239,13 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
     x2 = x if x.dim() == 2 else x.reshape(-1, bank.K)
     k = rhs_indices.shape[-1] if rhs_indices.dim() == 2 else 1
     R = rhs_indices.numel()
-    rhs = rhs_indices
-    if rhs.dtype is not torch.int32 or not rhs.is_contiguous():
-        rhs = rhs.to(torch.int32).contiguous()
+    rhs = expert_ids(rhs_indices, 0, bank.E)
     if lhs_indices is not None:
         lhs = lhs_indices.reshape(-1).to(torch.int64)
-        if lhs.numel() != R:
-            raise JangqError(_lib.JQ_EINVAL, "lhs_indices and rhs_indices differ in length")
-        x2, x_div = x2.index_select(0, lhs), 1
+        if lhs.numel() != R or (x2.shape[0] == 0 and R > 0):
+            raise JangqError(_lib.JQ_EINVAL, "lhs_indices and rhs_indices differ in length, or there are no rows of x")
+        # an index outside x names its first or last row: a read out of range would end the process
+        x2, x_div = x2.index_select(0, lhs.clamp(0, max(x2.shape[0] - 1, 0))), 1
     elif x2.shape[0] == R:
         x_div = 1
     elif rhs_indices.dim() == 2 and x2.shape[0] == rhs_indices.shape[0] and k > 0:

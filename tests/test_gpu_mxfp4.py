@@ -329,6 +329,13 @@ def test_gather_with_experts_elsewhere_and_all_on_one(pairs):
     for e in (0, 5, -1, E):
         _experts_close(jq.mxfp4_gather_matmul(x, wq, s, rhs_indices=torch.full_like(idx, e)), x, torch.full_like(idx, e), v, 1)
     assert jq.mxfp4_gather_matmul(x[:0], wq, s, rhs_indices=idx[:0]).shape == (0, N)
+    far = idx.long().clamp(0, E - 1)
+    far[::3] += 2 ** 32                                    # an expert of the bank in its low 32 bits
+    y = jq.mxfp4_gather_matmul(x, wq, s, rhs_indices=far)
+    assert not bool(y[::3].any()) and torch.equal(y[1::3], jq.mxfp4_gather_matmul(x, wq, s, rhs_indices=idx.clamp(0, E - 1))[1::3])
+    lhs = torch.arange(pairs, device="cuda") - 1           # -1 names the first row
+    y = jq.mxfp4_gather_matmul(x, wq, s, rhs_indices=idx, lhs_indices=lhs)
+    _experts_close(y, x[lhs.clamp(min=0)], idx, v, 1)
 
 
 def _silu(g):
@@ -464,7 +471,9 @@ def test_refusals():
              lambda: jq.mxfp4_gather_matmul(x[:, :64], bank, rhs_indices=idx), lambda: jq.mxfp4_gather_matmul(x.float(), bank, rhs_indices=idx),
              lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx[:1].reshape(-1)[:1]),
              lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx, lhs_indices=idx[0]),
-             lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, bank),
+             lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, bank), lambda: jq.moe_layer(x, idx[:, :0], idx[:, :0].float(), bank, bank, bank),
+             lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx.float()), lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx[:, :0]),
+             lambda: jq.mxfp4_gather_matmul(x[:0], bank, rhs_indices=idx, lhs_indices=idx),
              lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, None), lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, bank, return_slots=True)]
     for i, call in enumerate(calls):
         with pytest.raises(JangqError):
