@@ -131,9 +131,10 @@ struct ScaleGroup {
 #pragma unroll
         for (int j = 0; j < 4; ++j) row[j] = min(r0 + lane + 32 * j, last) * nblk;
     }
-    __device__ __forceinline__ void fetch(const uint8_t* base, int64_t total, int group, int nblk, bool vec) {
+    // from block b on, a multiple of 16
+    __device__ __forceinline__ void fetch(const uint8_t* base, int64_t total, int b, int nblk, bool vec) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load_scales32(base, total, row[j], group * 32, nblk, vec, v[j]);
+        for (int j = 0; j < 4; ++j) load_scales32(base, total, row[j], b, nblk, vec, v[j]);
     }
     // chunk c of stage i: to slot + i * STAGE + c * GAP
     template <int STAGE, int GAP> __device__ __forceinline__ void store(uint8_t* slot, int lane) const {
@@ -174,13 +175,16 @@ __device__ __forceinline__ void store_tile32(const Gemm4Args& a, const uint32_t 
     }
 }
 
-// ---- up to 128 activation rows: one tile per CTA, six stages ------------------------------------------------
+// ---- tiles of 128 weight rows x up to 128 activation rows, one per CTA ----------------------------------------
+// KS: CTAs of a cluster (along blockIdx.z) that split K where the tiles would leave most SMs idle: each leaves its sums as
+// float32 in its (by then idle) shared memory; after a cluster barrier CTA r adds and stores the activation rows of its share,
+// in rank order.  Both cluster barriers are reached by every thread on every path.
 constexpr int G4S_RA = 5, G4S_SF = 2 * 1024, G4S_THREADS = 256, G4S_DCOLS = 128, G4S_SFCOLS = 16, G4S_SETS = 3, G4S_SLOTS = 2 * G4S_SETS;
 constexpr size_t G4S_SMEM = 1024 + (size_t)G4S_RA * 2 * G4_A + G4S_SLOTS * G4_GS * G4S_SF + (2 * G4S_RA + 2 * G4S_SLOTS + 1) * 8 + 16;
 static_assert(G4S_SMEM <= 227 * 1024, "shared memory of one CTA");
 static_assert(G4S_DCOLS + 2 * G4_GS * G4S_SFCOLS <= G4_NCOLS, "tensor memory");
 
-template <typename OT>
+template <typename OT, int KS>
 __global__ void __launch_bounds__(G4S_THREADS, 1)
 mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Gemm4Args a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -194,8 +198,11 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accfull + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t n0 = (int64_t)blockIdx.x * 128;
-    const int rows = (int)a.M, nst = (a.nblk + 7) / 8;
+    const int64_t n0 = (int64_t)blockIdx.x * 128, m0 = (int64_t)blockIdx.y * a.tn;
+    const int rows = (int)min((int64_t)a.tn, a.M - m0);
+    // this CTA's stages [st0, st0 + nst): all, or its share of a split K, from an even one on (scales are read by 16 bytes)
+    const int all = (a.nblk + 7) / 8, rank = KS > 1 ? (int)blockIdx.z : 0;
+    const int st0 = rank * all / KS & ~1, nst = (rank == KS - 1 ? all : (rank + 1) * all / KS & ~1) - st0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < G4S_RA; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
@@ -220,8 +227,8 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
                 ok = ts_wait(empty + s, ph);
                 if (!ok) break;
                 mbar_expect_tx(full + s, bytes);                              // parts outside the matrices read as zeros
-                tma_load_2d(sA + s * G4_A, &wmap, i * 128, (int)n0, full + s);
-                tma_load_2d(sB + s * G4_A, &xmap, i * 128, 0, full + s);
+                tma_load_2d(sA + s * G4_A, &wmap, (st0 + i) * 128, (int)n0, full + s);
+                tma_load_2d(sB + s * G4_A, &xmap, (st0 + i) * 128, (int)m0, full + s);
                 if (++s == G4S_RA) { s = 0; ph ^= 1u; }
             }
         }
@@ -256,10 +263,10 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
         const uint8_t* base = part ? a.xscales : a.wscales;
         const int64_t count = part ? a.M : a.N;
         ScaleGroup sg;
-        sg.init(part ? 0 : n0, count - 1, a.nblk, lane);
+        sg.init(part ? m0 : n0, count - 1, a.nblk, lane);
         uint32_t ph = 1u;
         int slot = set;
-        if (set < ngrp) sg.fetch(base, count * a.nblk, set, a.nblk, a.vec);
+        if (set < ngrp) sg.fetch(base, count * a.nblk, st0 * 8 + set * 32, a.nblk, a.vec);
         for (int g = set; g < ngrp; g += G4S_SETS) {
             ok = __all_sync(0xFFFFFFFFu, ts_wait(sempty + slot, ph));
             if (!ok) break;
@@ -267,7 +274,7 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(sfull + slot);
             if ((slot += G4S_SETS) >= G4S_SLOTS) { slot = set; ph ^= 1u; }
-            if (g + G4S_SETS < ngrp) sg.fetch(base, count * a.nblk, g + G4S_SETS, a.nblk, a.vec);
+            if (g + G4S_SETS < ngrp) sg.fetch(base, count * a.nblk, st0 * 8 + (g + G4S_SETS) * 32, a.nblk, a.vec);
         }
         if (warp >= 4) {
             if (ok) ok = __all_sync(0xFFFFFFFFu, ts_wait(accfull, 0));
@@ -275,17 +282,45 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
                 tc_fence_after();
                 const int quarter = warp & 3;
                 const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16);
-                OT* y = reinterpret_cast<OT*>(a.y);
+                OT* y = reinterpret_cast<OT*>(a.y) + m0 * a.ldy;
 #pragma unroll 1
                 for (int c0 = 0; c0 < rows; c0 += 32) {
                     uint32_t v[32];
                     tmem_ld32(src + (uint32_t)c0, v);
+                    if constexpr (KS > 1) {
+                        float* out = reinterpret_cast<float*>(smem) + c0 * 128 + quarter * 32 + lane;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c0 + j < rows) out[j * 128] = __uint_as_float(v[j]);
+                        continue;
+                    }
                     store_tile32<OT>(a, v, y + c0 * a.ldy, rows - c0, n0 + quarter * 32 + lane, a.y_pair_ok && n0 + 128 <= a.N, lane);
                 }
             }
         }
     }
     __syncwarp();
+    if constexpr (KS > 1) {
+        static_assert(128 * 128 * 4 <= G4S_RA * 2 * G4_A, "staged sums fit");
+        ts_cluster_sync();                               // the staged sums are complete
+        const int t0 = rank * rows / KS, t1 = (rank + 1) * rows / KS;
+        for (int q = threadIdx.x + t0 * 32; q < t1 * 32; q += G4S_THREADS) {        // four neighbouring weight rows
+            const int tok = q >> 5, nl = (q & 31) * 4;
+            const float* src = reinterpret_cast<const float*>(smem) + tok * 128 + nl;
+            float4 f = ld_cluster_f32x4(src, 0);
+#pragma unroll
+            for (int r = 1; r < KS; ++r) {
+                const float4 o = ld_cluster_f32x4(src, (uint32_t)r);
+                f.x += o.x; f.y += o.y; f.z += o.z; f.w += o.w;
+            }
+            OT* yp = reinterpret_cast<OT*>(a.y) + (m0 + tok) * a.ldy + n0 + nl;
+            const float fv[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n0 + nl + j < a.N) yp[j] = Elt<OT>::from_f32(fv[j]);
+        }
+        ts_cluster_sync();                               // every CTA keeps its shared memory until all have read it
+    }
     if (!ok) atomicOr(a.status, JQ_STATUS_LOCAL_WAIT);
     tc_fence_before();
     const int gave_up = __syncthreads_or(ok ? 0 : 1);
@@ -469,7 +504,7 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
             if (fresh)
                 sg.init(part ? (int64_t)(tile % mt) * a.tn + (part - 1) * 128 : (int64_t)(tile / mt) * 256 + rank * 128, count - 1,
                         a.nblk, lane);
-            sg.fetch(base, count * a.nblk, g, a.nblk, a.vec);
+            sg.fetch(base, count * a.nblk, g * 32, a.nblk, a.vec);
         };
         uint32_t tile = first;
         int g = set;
@@ -584,6 +619,13 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(G4_NCOLS) : "memory");
 }
 
+// What the choice of a form goes by (us on B200; K stages of 256 codes).  One CTA per tile: 2 once, then per wave of tiles 2.2 and
+// 0.205 + 0.00085 tn per stage; a split of K adds 0.7 + 0.011 tn.  CTA pairs: 8.7 once, then 0.04 + 0.0015 tn per stage and round.
+// Measured: 16 rows 4096x4096 7.6 unsplit, 6.5 by 2, 6.0 by 4, 13.1 in pairs; 128 rows 2048x8192 12.7, 11.0, 9.0, 19.7; 256 rows
+// 4096x4096 9.0, 9.0, 15.4, 15.6; 1024 rows 4096x4096 16.0, 30.6, 53.5, 16.0; 4096 rows 14336x4096 181 unsplit, 97.5 in pairs.
+constexpr double G4_T_ONCE = 2.0, G4_T_WAVE = 2.2, G4_T_STAGE = 0.205, G4_T_ROW = 0.00085, G4_T_SPLIT = 0.7, G4_T_SPLIT_ROW = 0.011;
+constexpr double G4_T_PAIR = 8.7, G4_T_PSTAGE = 0.04, G4_T_PROW = 0.0015;
+
 static int encode_codes(CUtensorMap* map, const void* codes, int64_t rows, int64_t K, int box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();
     JQ_REQUIRE(enc != nullptr, JQ_ECUDA, "cuTensorMapEncodeTiled is not available from this driver");
@@ -598,9 +640,13 @@ static int encode_codes(CUtensorMap* map, const void* codes, int64_t rows, int64
     return JQ_OK;
 }
 
-template <typename OT, bool PAIR>
+// KS: CTAs that split K of a tile, 0: CTA pairs
+template <typename OT, int KS>
 static int launch_gemm4(const CUtensorMap& wmap, const CUtensorMap& xmap, const Gemm4Args& a, cudaStream_t st) {
-    auto kernel = PAIR ? mxfp4_gemm4_pair_kernel<OT> : mxfp4_gemm4_kernel<OT>;
+    constexpr bool PAIR = KS == 0;
+    void (*kernel)(CUtensorMap, CUtensorMap, Gemm4Args);
+    if constexpr (PAIR) kernel = mxfp4_gemm4_pair_kernel<OT>;
+    else kernel = mxfp4_gemm4_kernel<OT, KS>;
     constexpr size_t smem = PAIR ? G4P_SMEM : G4S_SMEM;
     static bool attr_done[64] = {};
     int dev = 0;
@@ -609,9 +655,23 @@ static int launch_gemm4(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
         JQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    const unsigned grid = PAIR ? (unsigned)(2 * std::min(a.tiles, sm_count() / 2)) : (unsigned)((a.N + 127) / 128);
-    kernel<<<grid, PAIR ? G4P_THREADS : G4S_THREADS, smem, st>>>(wmap, xmap, a);
-    return check_launch("mxfp4_gemm4");
+    if constexpr (PAIR) {
+        kernel<<<(unsigned)(2 * std::min(a.tiles, sm_count() / 2)), G4P_THREADS, smem, st>>>(wmap, xmap, a);
+        return check_launch("mxfp4_gemm4");
+    } else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.M + a.tn - 1) / a.tn), KS);
+        cfg.blockDim = dim3(G4S_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = KS;
+        cfg.attrs = attr;
+        cfg.numAttrs = KS > 1 ? 1 : 0;
+        JQ_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, a));
+        return JQ_OK;
+    }
 }
 
 }  // namespace jq
@@ -635,21 +695,32 @@ extern "C" int jq_mxfp4_gemm4(const uint32_t* xcodes, const uint8_t* xscales, in
     a.wscales = wscales; a.xscales = xscales; a.y = y;
     a.M = M; a.N = N; a.ldy = ldy;
     a.nblk = (int)(K / MX_BLOCK);
-    const bool pair = M > 128;
-    a.tn = (int)((M + 15) / 16 * 16);
-    if (pair) {
-        // tiles of 256 x tn in rounds of all pairs: a tile takes about tn + 24 (its first copies) times its stages
-        int64_t best = INT64_MAX;
-        const int64_t least = (M + G4P_TN - 1) / G4P_TN, pairs = sm_count() / 2, ncol = (N + 255) / 256;
-        for (int64_t nt = least; nt <= least + 3; ++nt) {
-            const int64_t tn = ((M + nt - 1) / nt + 15) / 16 * 16, tiles = (M + tn - 1) / tn * ncol;
-            const int64_t t = (tiles + pairs - 1) / pairs * (tn + 24);
-            if (t < best) { best = t; a.tn = (int)tn; }
+    // The form with the shortest estimated time (us).
+    const int64_t sms = sm_count(), nst = (a.nblk + 7) / 8;
+    int ks = 0;
+    double best = 1e30;
+    {
+        const int64_t mt = (M + 127) / 128, tn = ((M + mt - 1) / mt + 15) / 16 * 16, tiles = (M + tn - 1) / tn * ((N + 127) / 128);
+        for (int k : {1, 2, 4}) {
+            if ((M + tn - 1) / tn >= 65536 || (k > 1 && nst < 4 * k)) continue;
+            const int64_t slots = k == 4 ? sms / 37 * 8 : sms / k, waves = (tiles + slots - 1) / slots;      // a cluster stays within a GPC
+            const double t = G4_T_ONCE + waves * (G4_T_WAVE + (double)((nst + k - 1) / k) * (G4_T_STAGE + G4_T_ROW * tn) +
+                                                  (k > 1 ? G4_T_SPLIT + G4_T_SPLIT_ROW * tn : 0.0));
+            if (t < best) { best = t; ks = k; a.tn = (int)tn; }
         }
     }
-    const int64_t mt = (M + a.tn - 1) / a.tn, tiles = (N + 255) / 256 * mt;
-    JQ_REQUIRE(tiles < (1ll << 30), JQ_EUNSUPPORTED, "too many tiles for one launch (%lld)", (long long)tiles);
-    a.mt = (int)mt; a.tiles = (int)tiles;
+    int64_t pair_tiles = 0;
+    {
+        const int64_t least = (M + G4P_TN - 1) / G4P_TN, ncol = (N + 255) / 256;
+        for (int64_t nt = least; nt <= least + 3; ++nt) {
+            const int64_t tn = ((M + nt - 1) / nt + 15) / 16 * 16, mt = (M + tn - 1) / tn, tiles = mt * ncol;
+            const double t = G4_T_PAIR + (double)((tiles + sms / 2 - 1) / (sms / 2)) * nst * (G4_T_PSTAGE + G4_T_PROW * tn);
+            if (t < best) { best = t; ks = 0; a.tn = (int)tn; a.mt = (int)mt; pair_tiles = tiles; }
+        }
+    }
+    const bool pair = ks == 0;
+    JQ_REQUIRE(!pair || pair_tiles < (1ll << 30), JQ_EUNSUPPORTED, "too many tiles for one launch (%lld)", (long long)pair_tiles);
+    a.tiles = (int)pair_tiles;
     a.vec = a.nblk % 16 == 0 && aligned(wscales, 16) && aligned(xscales, 16);
     a.y_pair_ok = (aligned(y, 4) && ldy % 2 == 0) ? 1 : 0;
     a.status = status_word();
@@ -659,7 +730,10 @@ extern "C" int jq_mxfp4_gemm4(const uint32_t* xcodes, const uint8_t* xscales, in
     if (rc != JQ_OK) return rc;
     rc = encode_codes(&xmap, xcodes, M, K, pair ? a.tn / 2 : a.tn);
     if (rc != JQ_OK) return rc;
-    JQ_DISPATCH_DTYPE(y_dtype, OT, return pair ? launch_gemm4<OT, true>(wmap, xmap, a, (cudaStream_t)stream)
-                                               : launch_gemm4<OT, false>(wmap, xmap, a, (cudaStream_t)stream));
+    JQ_DISPATCH_DTYPE(y_dtype, OT,
+        if (ks == 1) return launch_gemm4<OT, 1>(wmap, xmap, a, (cudaStream_t)stream);
+        if (ks == 2) return launch_gemm4<OT, 2>(wmap, xmap, a, (cudaStream_t)stream);
+        if (ks == 4) return launch_gemm4<OT, 4>(wmap, xmap, a, (cudaStream_t)stream);
+        return launch_gemm4<OT, 0>(wmap, xmap, a, (cudaStream_t)stream))
     return JQ_OK;
 }

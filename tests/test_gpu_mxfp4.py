@@ -173,7 +173,9 @@ def test_gemm(M, N, K, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 128, 64), (2, 200, 96), (16, 333, 256), (17, 128, 288), (33, 257, 1056), (128, 130, 512),
-                                   (129, 64, 2080), (255, 129, 320), (256, 256, 1024), (300, 72, 4128), (520, 1000, 640)])
+                                   (129, 64, 2080), (255, 129, 320), (256, 256, 1024), (300, 72, 4128), (520, 1000, 640),
+                                   (5, 130, 8224), (128, 100, 4128), (130, 2100, 2112), (700, 5000, 288), (2100, 4101, 320),
+                                   (1100, 9000, 1056), (2500, 4352, 288)])
 def test_both_operands_quantized(M, N, K, out):
     wq, s, v = _packed(M + N + K, (N, K))
     xq, xs, xv = _packed(K, (M, K), 1.0)
