@@ -346,24 +346,26 @@ qgemm_ts_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
         // ---------------- MMA issuer ----------------
         const uint32_t idesc = umma_idesc_ts<AT>(n_mma);
         const uint32_t x_lo = umma_desc_sw128_lo(smem_u32(sX));
-        int s = 0;
-        uint32_t ph = 0u;
-        for (int i = 0; i < nkb; ++i) {
-            ok = __all_sync(0xFFFFFFFFu, ts_wait(full + s, ph));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t xd = x_lo + (uint32_t)s * (uint32_t)(C::X_STAGE >> 4);
-            const uint32_t ac = tmem_base + (uint32_t)(C::ACOL + s * 32);
-            if (elect_one()) {
+        // one thread runs the loop: with the whole warp in it (votes, an election per k-block) issuing a k-block took 350 ns,
+        // more than its MMAs run
+        if (elect_one()) {
+            int s = 0;
+            uint32_t ph = 0u;
+            for (int i = 0; i < nkb; ++i) {
+                ok = ts_wait(full + s, ph);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t xd = x_lo + (uint32_t)s * (uint32_t)(C::X_STAGE >> 4);
+                const uint32_t ac = tmem_base + (uint32_t)(C::ACOL + s * 32);
 #pragma unroll
                 for (int k = 0; k < GEMM_BK / 16; ++k)
-                    umma_f16_ts(tmem_base, ac + k * 8, umma_desc_join(xd + k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                    umma_f16_ts(tmem_base, ac + k * 8, umma_desc_join(xd + k * 2), idesc, k > 0 ? 1u : (uint32_t)i);
                 umma_commit(empty + s);
-                if (i == nkb - 1) umma_commit(accfull);
+                if (++s == RA) { s = 0; ph ^= 1u; }
             }
-            __syncwarp();
-            if (++s == RA) { s = 0; ph ^= 1u; }
+            if (ok) umma_commit(accfull);
         }
+        ok = __all_sync(0xFFFFFFFFu, ok);
     } else if (warp < 4) {
         // ---------------- code loaders ----------------
         int buf = 0, slot = 0;
@@ -611,32 +613,32 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         const uint32_t x_lo = umma_desc_sw128_lo(smem_u32(sX));
-        int s = 0, d = 0;
-        uint32_t ph = 0u, dph = 1u;
-        for (int tile = first; tile < total && ok; tile += step) {
-            const PersTile t = take(tile);
-            if (t.rows <= 0) continue;
-            const uint32_t idesc = umma_idesc_ts<AT>((t.rows + 15) & ~15);
-            const uint32_t dcol = tmem_base + (uint32_t)(d * C::TNMAX);
-            ok = __all_sync(0xFFFFFFFFu, ts_wait(accempty + d, dph));
-            for (int i = 0; i < nkb && ok; ++i) {
-                ok = __all_sync(0xFFFFFFFFu, ts_wait(full + s, ph));
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t xd = x_lo + (uint32_t)s * (uint32_t)(C::X_STAGE >> 4);
-                const uint32_t ac = tmem_base + (uint32_t)(C::ACOL + s * 32);
-                if (elect_one()) {
+        if (elect_one()) {                                     // one thread, as in the one-tile form
+            int s = 0, d = 0;
+            uint32_t ph = 0u, dph = 1u;
+            for (int tile = first; tile < total && ok; tile += step) {
+                const PersTile t = take(tile);
+                if (t.rows <= 0) continue;
+                const uint32_t idesc = umma_idesc_ts<AT>((t.rows + 15) & ~15);
+                const uint32_t dcol = tmem_base + (uint32_t)(d * C::TNMAX);
+                ok = ts_wait(accempty + d, dph);
+                for (int i = 0; i < nkb && ok; ++i) {
+                    ok = ts_wait(full + s, ph);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t xd = x_lo + (uint32_t)s * (uint32_t)(C::X_STAGE >> 4);
+                    const uint32_t ac = tmem_base + (uint32_t)(C::ACOL + s * 32);
 #pragma unroll
                     for (int k = 0; k < GEMM_BK / 16; ++k)
-                        umma_f16_ts(dcol, ac + k * 8, umma_desc_join(xd + k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                        umma_f16_ts(dcol, ac + k * 8, umma_desc_join(xd + k * 2), idesc, k > 0 ? 1u : (uint32_t)i);
                     umma_commit(empty + s);
-                    if (i == nkb - 1) umma_commit(accfull + d);
+                    if (++s == RA) { s = 0; ph ^= 1u; }
                 }
-                __syncwarp();
-                if (++s == RA) { s = 0; ph ^= 1u; }
+                if (ok) umma_commit(accfull + d);
+                if (++d == C::ND) { d = 0; dph ^= 1u; }
             }
-            if (++d == C::ND) { d = 0; dph ^= 1u; }
         }
+        ok = __all_sync(0xFFFFFFFFu, ok);
     } else if (warp < 4) {
         // ---------------- code loaders ----------------
         int buf = 0, slot = 0;
