@@ -16,6 +16,10 @@
 // goes through a batch of tiles with one stretch of k, whose activations stay in registers, and then with its next one; its
 // sums stand in shared memory until the CTA meets at the end of the batch to add them, KS to a row, in an order that does not
 // change.
+//
+// Measured (bf16, copies in turn beyond L2): one row of 14336 x 4096 11.0 us = 2.8 TB/s, 11008 x 4096 9.3, 4096 x 4096 6.2,
+// 2048 x 2048 4.1; eight rows 16.7, 14.4, 9.5, 5.8.  The large ones are bound by issue (half of the scheduler's slots, no pipe
+// above a third) in four warps per scheduler, the small ones by some 3 us of launch, staging and the meeting at the end.
 #include <algorithm>
 
 #include "jq_launch.cuh"
@@ -62,11 +66,21 @@ static_assert(MXV_RING + mxv_part<false>() + MXV_EXTRA + (MXV_MAX_K + MXV_PAD) *
 // each, fall into eight bank groups.
 __device__ __forceinline__ int mxv_chunk(int b, int row) { return b ^ ((row & 1) << 2 | (row >> 1 & 3)); }
 
-// 2^(byte - 127), half h of a 16-bit pair of scale bytes
-__device__ __forceinline__ float mx_scale(uint32_t pair, int h, bool fast) {
-    const uint32_t f = (h ? pair << 15 : pair << 23) & 0x7F800000u;
-    if (fast) return __uint_as_float(f);
+// 2^(byte - 127) of byte I of a word; the other form also of bytes 0 (a subnormal) and 255 (not a number)
+template <int I> __device__ __forceinline__ float mx_scale(uint32_t w) {
+    return __uint_as_float((I < 3 ? w << (23 - 8 * I) : w >> 1) & 0x7F800000u);
+}
+template <int I> __device__ __forceinline__ float mx_scale_any(uint32_t w) {
+    const uint32_t f = __float_as_uint(mx_scale<I>(w));
     return __uint_as_float(f == 0u ? 0x00400000u : (f == 0x7F800000u ? 0x7FC00000u : f));
+}
+// the four of a word; fast: none of the warp's bytes is 0 or 255
+__device__ __forceinline__ void mx_scales4(uint32_t w, bool fast, float (&f)[4]) {
+    if (fast) {
+        f[0] = mx_scale<0>(w); f[1] = mx_scale<1>(w); f[2] = mx_scale<2>(w); f[3] = mx_scale<3>(w);
+    } else {
+        f[0] = mx_scale_any<0>(w); f[1] = mx_scale_any<1>(w); f[2] = mx_scale_any<2>(w); f[3] = mx_scale_any<3>(w);
+    }
 }
 // eight codes -> four f16 pairs of their plain values, in order
 __device__ __forceinline__ void mx_values8(uint32_t w, uint32_t (&o)[4]) {
@@ -119,6 +133,7 @@ template <bool COLS, bool GATHER> struct MxvAhead {
     uint32_t item, base, stop;           // of the batch [base, stop)
     int u, left;                         // left: N - 1 - first of the 16 weight rows; rows past it repeat the last one
     bool none;                           // no expert of the bank takes the pair
+    int bytes;                           // of scales from there to the end of the array, at most 2^30
     const uint8_t *codes, *scales;       // of the first of the 16 rows
     __device__ __forceinline__ uint32_t batch_end(const MxGemvArgs& a, uint32_t end) const {
         return min(base + mxv_batch<COLS>(), GATHER ? min(end, (base / a.tiles + 1) * a.tiles) : end);
@@ -138,12 +153,14 @@ template <bool COLS, bool GATHER> struct MxvAhead {
         left = (int)(a.N - 1 - n0);
         codes = a.codes + (row + n0) * a.nblk * 16;
         scales = a.scales + (row + n0) * a.nblk;
+        bytes = (int)min(a.scale_bytes - (row + n0) * a.nblk, (int64_t)1 << 30);
     }
     __device__ __forceinline__ void next(const MxGemvArgs& a, uint32_t end, int nunit, int ks, int KS, int rg, int rows) {
         if (++item < stop) {
             left -= rows;
             codes += (int64_t)rows * a.nblk * 16;
             scales += (int64_t)rows * a.nblk;
+            bytes = (int)min(a.scale_bytes - (scales - a.scales), (int64_t)1 << 30);
             return;
         }
         if ((u += KS) >= nunit) {
@@ -177,6 +194,7 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
     const int crow = a.nblk * 16;
     const uint32_t begin = (uint32_t)((uint64_t)a.items * blockIdx.x / gridDim.x), end = (uint32_t)((uint64_t)a.items * (blockIdx.x + 1) / gridDim.x);
 
+    const bool three = a.nblk & 3;
     // one stretch into a slot of the ring; codes of zero past the row's end and without an expert
     MxvAhead<COLS, GATHER> ahead{};
     const uint32_t cdst = smem_u32(ring) + (uint32_t)((lane >> 3) * 128), sdst = smem_u32(ring) + MXV_CODES;
@@ -193,17 +211,15 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                              ::"r"(cdst + at + (uint32_t)(c * 512 + mxv_chunk(lane & 7, r) * 16)),
                                "l"(src + (int64_t)min(r, ahead.left) * crow), "r"(in ? 16 : 0) : "memory");
             }
-            // the words around a row's eight bytes; the array's last one may be short
-            const uintptr_t last = reinterpret_cast<uintptr_t>(a.scales) + a.scale_bytes;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = lane & 15, w = (lane >> 4) + 2 * i;
-                const uintptr_t word =
-                    (reinterpret_cast<uintptr_t>(ahead.scales + (int64_t)min(r, ahead.left) * a.nblk + ahead.u * MXV_UNIT) & ~(uintptr_t)3) + 4 * w;
-                if (w < 3 && word < last)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
-                                 ::"r"(sdst + at + (uint32_t)(r * 16 + w * 4)), "l"(word), "r"((int)min(last - word, (uintptr_t)4)) : "memory");
-            }
+            // the aligned words around a row's eight bytes (two where rows are whole words); the array's last one may be short
+            const int off = min(lane & 15, ahead.left) * a.nblk + ahead.u * MXV_UNIT + (lane >> 4) * 4;
+            const int low = (int)(reinterpret_cast<uintptr_t>(ahead.scales) + off) & 3, have = ahead.bytes - (off - low);
+            const uint8_t* word = ahead.scales + (off - low);
+            const uint32_t wdst = sdst + at + (uint32_t)((lane & 15) * 16 + (lane >> 4) * 4);
+            if (have > 0)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(wdst), "l"(word), "r"(min(have, 4)) : "memory");
+            if (three && lane < 16 && have > 8)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(wdst + 8), "l"(word + 8), "r"(min(have - 8, 4)) : "memory");
             ahead.next(a, end, nunit, ks, KS, rg, rows);
         }
         cp_async_commit();
@@ -236,6 +252,7 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
     const float* sel = COLS ? se + min(t >> 1, M - 1) * nb + 2 * (t & 1) : se + 2 * t;
     // offset of this lane's codes, and of the scale bytes of its rows, in a slot
     const uint8_t* codes0 = ring + g * 128;
+    const uint32_t pick = t & 1 ? 0x7632u : 0x5410u;       // this lane's two of four blocks, in two rows' words
 
     int slot = 0;
     for (uint32_t item = begin; item < end;) {
@@ -313,12 +330,13 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         // columns 2t, 2t + 1: blocks 2 (t & 1), + 1 of the four, token t / 2
-                        const uint32_t s0 = t & 1 ? p0[h] >> 16 : p0[h], s1 = t & 1 ? p1[h] >> 16 : p1[h];
                         if constexpr (SCALED) {
                             d[h][0] *= xe[h].x; d[h][1] *= xe[h].y; d[h][2] *= xe[h].x; d[h][3] *= xe[h].y;
                         }
-                        v0 = fmaf(d[h][1], mx_scale(s0, 1, fast), fmaf(d[h][0], mx_scale(s0, 0, fast), v0));
-                        v1 = fmaf(d[h][3], mx_scale(s1, 1, fast), fmaf(d[h][2], mx_scale(s1, 0, fast), v1));
+                        float f[4];                        // rows g and g + 8 of the two blocks
+                        mx_scales4(prmt(p0[h], p1[h], pick), fast, f);
+                        v0 = fmaf(d[h][1], f[1], fmaf(d[h][0], f[0], v0));
+                        v1 = fmaf(d[h][3], f[3], fmaf(d[h][2], f[2], v1));
                     }
                     // the two column pairs of a token
                     v0 += __shfl_xor_sync(0xFFFFFFFFu, v0, 1);
@@ -329,7 +347,15 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                         o[8] = u == ks ? v1 : o[8] + v1;
                     }
                 } else {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f}, f0[MXV_UNIT], f1[MXV_UNIT];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float f[4];
+                        mx_scales4(p0[i], fast, f);
+                        f0[4 * i] = f[0]; f0[4 * i + 1] = f[1]; f0[4 * i + 2] = f[2]; f0[4 * i + 3] = f[3];
+                        mx_scales4(p1[i], fast, f);
+                        f1[4 * i] = f[0]; f1[4 * i + 1] = f[1]; f1[4 * i + 2] = f[2]; f1[4 * i + 3] = f[3];
+                    }
 #pragma unroll
                     for (int b = 0; b < MXV_UNIT; ++b) {   // lane t has eight codes of block b
                         uint32_t e0[4], e1[4];
@@ -339,15 +365,13 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                         float d[4];
                         H::mma0(d, fa, xv[b].x, xv[b].y);
                         H::mma(d, fb, xv[b].z, xv[b].w);
-                        const uint32_t s0 = b & 2 ? p0[b >> 2] >> 16 : p0[b >> 2], s1 = b & 2 ? p1[b >> 2] >> 16 : p1[b >> 2];
-                        const float f0 = mx_scale(s0, b & 1, fast), f1 = mx_scale(s1, b & 1, fast);
                         if constexpr (SCALED) {
                             d[0] *= xe[b].x; d[1] *= xe[b].y; d[2] *= xe[b].x; d[3] *= xe[b].y;
                         }
-                        acc[0] = fmaf(d[0], f0, acc[0]);
-                        acc[1] = fmaf(d[1], f0, acc[1]);
-                        acc[2] = fmaf(d[2], f1, acc[2]);
-                        acc[3] = fmaf(d[3], f1, acc[3]);
+                        acc[0] = fmaf(d[0], f0[b], acc[0]);
+                        acc[1] = fmaf(d[1], f0[b], acc[1]);
+                        acc[2] = fmaf(d[2], f1[b], acc[2]);
+                        acc[3] = fmaf(d[3], f1[b], acc[3]);
                     }
                     // rows g, g + 8 of tokens 2t, 2t + 1
                     float* o = out + 2 * t * 17 + g;
