@@ -301,9 +301,10 @@ def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch
     # the pitch of a single row says nothing, and a broadcast one (0) names no rows
     if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
         logits = logits.contiguous()
-    # sizes a table cannot have are refused by the library; nothing of theirs is allocated before
-    idx = logits.new_empty((T, max(k, 0)), dtype=torch.int32)
-    w = logits.new_empty((T, max(k, 0)), dtype=torch.float32)
+    if not 1 <= k <= E:                  # here, before a table of that size is asked for
+        raise JangqError(_lib.JQ_EINVAL, f"k must be 1 to the number of experts ({E}), got {k}")
+    idx = logits.new_empty((T, k), dtype=torch.int32)
+    w = logits.new_empty((T, k), dtype=torch.float32)
     with _lib.on_device(dev):
         _lib.check(lib.jq_moe_route_topk(logits.data_ptr(), _lib.dtype_id(logits.dtype), logits.stride(0) if T > 1 else E, T, E,
                                          k, _SCORES[score], bias.data_ptr() if bias is not None else None, groups, groups_kept,

@@ -18,8 +18,8 @@ from ._lib import JangqError
 BLOCK = 32
 SORT_THRESHOLD = 64      # pairs; as gather_qmm
 # Rows that the mat-vec takes in one launch (their activations in shared memory: rows * K up to MXFP4_GEMV_MAX_K).  Beyond,
-# every weight is read again, and the tensor-core GEMM is faster: 8 rows of 14336x4096 17 us here, 23 there; 16 rows 57 and 23;
-# 2 rows of 4096x14336 16 and 21, 4 rows 30 and 21.
+# every weight is read again, and the tensor-core GEMM is faster: 8 rows of 14336x4096 16.7 us here, 22.2 there, 9 rows 29 and
+# 22; 8 rows of 2048x2048 5.8 and 6.6, 9 rows 10 and 6.7; 2 rows of 4096x14336 15.2 and 20.7, 4 rows 29 and 21.
 MATVEC_ROWS = 8
 
 
@@ -177,14 +177,19 @@ class MXFP4ExpertBank:
         return self.gemm_ok and self.E <= 4096 and (pairs >= SORT_THRESHOLD or self.K > _lib.MXFP4_GEMV_MAX_K)
 
 
+def _check_integers(idx: torch.Tensor, what: str):
+    if idx.is_floating_point() or idx.is_complex() or idx.dtype in (torch.bool, torch.uint64):
+        raise JangqError(_lib.JQ_EINVAL, f"{what} must be integers of up to 64 bits with a sign, got {idx.dtype}")
+
+
 def expert_ids(idx: torch.Tensor, base: int, experts: int) -> torch.Tensor:
     """Contiguous int32 expert ids of the pairs; ids beyond 32 bits stay outside [base, base + experts)."""
     if idx.dtype is torch.int32:
         return idx if idx.is_contiguous() else idx.contiguous()
     if idx.dtype is torch.int64:
         idx = idx.clamp(base - 1, base + experts)
-    elif idx.is_floating_point() or idx.is_complex() or idx.dtype is torch.bool:
-        raise JangqError(_lib.JQ_EINVAL, f"expert indices must be integers, got {idx.dtype}")
+    else:
+        _check_integers(idx, "expert indices")
     return idx.to(torch.int32).contiguous()
 
 
@@ -223,7 +228,7 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
     """y[r] = x[lhs[r]] . deq(w[rhs[r]])^T for stacked MXFP4 experts w [E, N, K/8], scales [E, N, K/32] (or an
     MXFP4ExpertBank): gather_qmm's call shape, indices and result [R, N] (x [R0, K]; rhs_indices [R] or [T, k]; without
     lhs_indices row r of x is used when R0 == R, row r // k when rhs is [T, k] with R0 == T).  Indices outside the bank
-    give rows of zeros.  Below 64 rows one mat-vec per row, above that the grouped tensor-core product."""
+    give rows of zeros; lhs indices outside x take its first or last row.  Below 64 rows one mat-vec per row, above that the grouped tensor-core product."""
     if rhs_indices is None:
         raise JangqError(_lib.JQ_EINVAL, "mxfp4_gather_matmul needs rhs_indices")
     if sorted_indices and lhs_indices is None:
@@ -241,6 +246,7 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
     R = rhs_indices.numel()
     rhs = expert_ids(rhs_indices, 0, bank.E)
     if lhs_indices is not None:
+        _check_integers(lhs_indices, "lhs_indices")
         lhs = lhs_indices.reshape(-1).to(torch.int64)
         if lhs.numel() != R or (x2.shape[0] == 0 and R > 0):
             raise JangqError(_lib.JQ_EINVAL, "lhs_indices and rhs_indices differ in length, or there are no rows of x")

@@ -476,6 +476,8 @@ def test_refusals():
              lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, bank), lambda: jq.moe_layer(x, idx[:, :0], idx[:, :0].float(), bank, bank, bank),
              lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx.float()), lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx[:, :0]),
              lambda: jq.mxfp4_gather_matmul(x[:0], bank, rhs_indices=idx, lhs_indices=idx),
+             lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx, lhs_indices=idx.float()),
+             lambda: jq.mxfp4_gather_matmul(x, bank, rhs_indices=idx.to(torch.uint64)),
              lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, None), lambda: jq.moe_layer(x, idx, idx.float(), bank, bank, bank, return_slots=True)]
     for i, call in enumerate(calls):
         with pytest.raises(JangqError):

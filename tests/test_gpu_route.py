@@ -107,7 +107,7 @@ def test_views_streams_and_graphs():
 @pytest.mark.parametrize("kw", [dict(k=0), dict(k=65), dict(k=9, groups=8, groups_kept=1), dict(k=2, groups=5), dict(k=2, groups=0),
                                 dict(k=2, groups=64), dict(k=2, groups=8, groups_kept=9), dict(k=2, groups=8, groups_kept=0),
                                 dict(k=2, groups=8, groups_kept=2, group_top=3), dict(k=2, groups=8, groups_kept=2, group_top=0),
-                                dict(k=2, score="relu"), dict(k=-1)])
+                                dict(k=2, score="relu"), dict(k=-1), dict(k=1 << 40), dict(k=(1 << 32) + 2)])
 def test_refusals(kw):
     logits = torch.zeros((3, 64), device="cuda")
     with pytest.raises(JangqError):
