@@ -1,4 +1,4 @@
-// Microscaled 4-bit floating point (OCP MX): 32 numbers share a power of two 2^(byte - 127), a number is e2m1: sign, two
+// Shared by the MXFP4 kernels.  Microscaled 4-bit floating point (OCP MX): 32 numbers share a power of two 2^(byte - 127), a number is e2m1: sign, two
 // exponent bits, one mantissa bit, values 0 .5 1 1.5 2 3 4 6.  Byte 255 marks a block that is not a number.
 #pragma once
 
@@ -18,7 +18,6 @@ int check_mxfp4_shape(int64_t rows, int64_t K);
 template <typename AT> struct Mx;
 template <> struct Mx<__nv_bfloat16> {
     static constexpr int POS = 6;                        // bit of the code's mantissa bit
-    static constexpr uint32_t MASK = 0x01C001C0u;
     static constexpr int FAST_MAX = 128;                 // largest byte whose lift is a bf16 number
     // 2^(byte - 1), twice
     __device__ static __forceinline__ uint32_t lift(uint32_t b) { return ((b + 126u) << 7) * 0x00010001u; }
@@ -31,7 +30,6 @@ template <> struct Mx<__nv_bfloat16> {
 };
 template <> struct Mx<__half> {
     static constexpr int POS = 9;
-    static constexpr uint32_t MASK = 0x0E000E00u;
     static constexpr int FAST_MAX = 128;
     // 2^(byte - 113), twice; zero below 2^-24, where no weight of the block reaches half of f16's smallest number
     __device__ static __forceinline__ uint32_t lift(uint32_t b) {
@@ -47,18 +45,10 @@ template <> struct Mx<__half> {
     }
 };
 
-// code fields (j, j + 4) of a word of eight codes, j = 0 .. 3: sign at bit 15, the rest at POS
-template <typename AT, int J>
-__device__ __forceinline__ uint32_t mx_field(uint32_t w) {
-    constexpr int up = 12 - 4 * J, at = Mx<AT>::POS - 4 * J;
-    const uint32_t s = up > 0 ? w << up : w;
-    const uint32_t m = at >= 0 ? w << at : w >> -at;
-    return (s & 0x80008000u) | (m & Mx<AT>::MASK);
-}
 // The eight magnitudes of a block, scaled, as the byte tables of two byte permutes: a code's three low bits are a permute
 // selector as they stand, so four codes cost a look-up of their high and one of their low bytes, and the scale is
 // multiplied in once per block instead of once per pair.  15 instructions per eight codes and 10 per block; fields shifted
-// into place and multiplied (mx_field) took 23 to the same order.
+// into place and multiplied took 23 to the same order.
 template <typename AT> struct MxTable {
     uint32_t h0, h1, l0, l1;
     // fast: the byte is at most FAST_MAX (in all lanes of the warp, which branch together)
