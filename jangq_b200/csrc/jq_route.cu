@@ -15,6 +15,9 @@
 // (the whole token again in float64: 22 us for 4096 x 256).  Where c grows with the logit alone (no bias, and at most the
 // best expert of a group counts) the order of the logits is the order of the scores, exactly.  A NaN logit counts as -inf, a
 // score of zero; +inf takes the limit.
+// Measured: one token, 128 experts, softmax 2.3 us (an empty launch is 2); 61 tokens, 512 experts, bias, 10 of them 6.8; sigmoid,
+// bias, the best 4 of 8 groups of 32, 8 experts: 592 tokens 5.5, 4096 tokens 13.8 (latency up to one token per scheduler, then issue
+// of the selections, the groups and the scores in like parts).
 #include "jq_launch.cuh"
 
 namespace jq {
@@ -95,6 +98,7 @@ struct RouteArgs {
     float* w;
     int T, E, k, sigmoid, groups, kept, top, renorm;
     int per;                         // experts of a group
+    int lanes_log2;                  // lanes of the warp per group: as many as fit
     float scale;
 };
 
@@ -105,17 +109,16 @@ template <typename LT> __device__ __forceinline__ float load_logit(const RouteAr
 // exp(l - mx) without inf - inf
 __device__ __forceinline__ double exp_below(float l, float mx) { return l == mx ? (mx == -INFINITY ? 0.0 : 1.0) : exp((double)l - (double)mx); }
 
-// Which groups stay, as a bit per group, from the choice scores of the token in shared memory.  near: set (in every lane)
+// Which groups stay, as a bit for each of a group's 1 << lanes_log2 lanes, from the choice scores of the token in shared memory.  near: set (in every lane)
 // when a group at the cut is within `close` of another.
 template <typename V>
 __device__ __forceinline__ uint32_t kept_groups(const RouteArgs& a, const V* row, int lane, float close, bool& near) {
-    // L lanes per group (a power of two): two largest of the lane's share, then a butterfly over the L lanes
-    int L = 1;
-    while (2 * L * a.groups <= 32) L *= 2;
-    const int g = lane / L;
+    // L lanes per group: two largest of the lane's share, then a butterfly over the L lanes
+    const int L = 1 << a.lanes_log2, g = lane >> a.lanes_log2;
     V best = -(V)INFINITY, second = -(V)INFINITY;
     if (g < a.groups)
-        for (int j = lane % L; j < a.per; j += L) {
+#pragma unroll 8
+        for (int j = lane & (L - 1); j < a.per; j += L) {
             const V v = row[g * a.per + j];
             second = v > best ? best : (v > second ? v : second);
             best = v > best ? v : best;
@@ -132,16 +135,13 @@ __device__ __forceinline__ uint32_t kept_groups(const RouteArgs& a, const V* row
     int rank = 0;
     bool touch = false;
     for (int o = 0; o < a.groups; ++o) {
-        const auto other = __shfl_sync(0xFFFFFFFFu, mine, o * L);
-        const V value = __shfl_sync(0xFFFFFFFFu, score, o * L);
+        const auto other = __shfl_sync(0xFFFFFFFFu, mine, o << a.lanes_log2);
+        const V value = __shfl_sync(0xFFFFFFFFu, score, o << a.lanes_log2);
         rank += (other > mine || (other == mine && o < g)) ? 1 : 0;
         touch |= o != g && !(fabs(value - score) > (V)close);            // two infinities differ by NaN, which is near
     }
     near = __any_sync(0xFFFFFFFFu, g < a.groups && touch && (rank == a.kept - 1 || rank == a.kept));
-    const uint32_t in = __ballot_sync(0xFFFFFFFFu, g < a.groups && rank < a.kept);      // L equal bits per group
-    uint32_t keep = 0;
-    for (int o = 0; o < a.groups; ++o) keep |= ((in >> (o * L)) & 1u) << o;
-    return keep;
+    return __ballot_sync(0xFFFFFFFFu, g < a.groups && rank < a.kept);
 }
 
 // Results of up to 32 selections from j0 on: lane j holds expert `mine`.  Returns the sum of their scores.
@@ -255,7 +255,7 @@ __device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int l
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = lane + 32 * i;
-        key[i] = e < E && (keep >> (int)(((float)e + 0.5f) * per_group) & 1u) ? order_key(c[i]) : 0u;
+        key[i] = e < E && (keep >> ((int)(((float)e + 0.5f) * per_group) << a.lanes_log2) & 1u) ? order_key(c[i]) : 0u;
     }
     uint32_t best, before = 0;
     int bi;                                                // register index of the lane's best
@@ -328,7 +328,7 @@ __device__ __noinline__ void route_token_exact(const RouteArgs& a, int64_t t, in
     uint64_t best = 0;
     int at = 0;
     for (int e = lane; e < a.E; e += 32) {
-        const uint64_t k = a.groups == 1 || (keep >> (e / a.per) & 1u) ? order_key(row[e]) : 0ull;
+        const uint64_t k = a.groups == 1 || (keep >> (e / a.per << a.lanes_log2) & 1u) ? order_key(row[e]) : 0ull;
         key[e] = k;
         if (k > best) { best = k; at = e; }
     }
@@ -428,6 +428,8 @@ extern "C" int jq_moe_route_topk(const void* logits, int logits_dtype, int64_t l
     // all groups kept is no grouping
     a.groups = groups_kept == groups ? 1 : groups;
     a.per = num_experts / a.groups;
+    a.lanes_log2 = 0;
+    while (a.groups > 1 && a.groups << (a.lanes_log2 + 1) <= 32) ++a.lanes_log2;
     a.kept = groups_kept; a.top = group_top; a.renorm = renorm; a.scale = scale;
     const bool screen = bias != nullptr || (a.groups > 1 && group_top == 2);
     JQ_DISPATCH_DTYPE(logits_dtype, LT, return launch_route_e<LT>(a, screen, (cudaStream_t)stream));
