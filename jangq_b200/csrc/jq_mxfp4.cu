@@ -116,8 +116,7 @@ __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* _
         const int64_t i = i0 + u * 256;
         if (i >= units) break;
         const uint32_t w = ws[u], b = bs[u];
-        // 2^(b - 127) as f32: byte 0 is a subnormal, 255 not a number
-        const float scale = __uint_as_float(b == 0u ? 0x00400000u : (b == 255u ? 0x7FC00000u : b << 23));
+        const float scale = mx_scale_f32(b);
         float v[NUM];
 #pragma unroll
         for (int j = 0; j < NUM / 2; ++j) {                                // two codes of a byte, as f16 numbers

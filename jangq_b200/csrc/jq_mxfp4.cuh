@@ -12,67 +12,67 @@ constexpr int MX_BLOCK = 32;
 int check_mxfp4_shape(int64_t rows, int64_t K);
 
 // ---- expansion to a 16-bit float type -----------------------------------------------------------------
-// The three low bits of a code placed at the top of the type's mantissa and the bottom of its exponent read as the code's
-// value times 2^-126 (bf16) or 2^-14 (f16), zero and the subnormal 0.5 included, so the scale goes in with the multiply
-// that lifts them: one product per two weights, and nothing is rounded where the type holds the weight.
+// eight codes -> four f16 pairs of their plain values, in order
+__device__ __forceinline__ void mx_values8(uint32_t w, uint32_t (&o)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+        : "r"(w));
+}
+// 2^(byte - 127) as f32: byte 0 is a subnormal, 255 not a number
+__device__ __forceinline__ float mx_scale_f32(uint32_t byte) {
+    return __uint_as_float(byte == 0u ? 0x00400000u : (byte == 255u ? 0x7FC00000u : byte << 23));
+}
+
+// One product per pair puts the scale in, rounded once where the type does not hold the weight.  FAST_MIN .. FAST_MAX: the bytes
+// whose factor is a number of the type.
 template <typename AT> struct Mx;
+// bf16: the three low bits of a code placed at the top of the mantissa and the bottom of the exponent read as the code's value
+// times 2^-126, zero and the subnormal 0.5 included.  A multiplication by 2^6 + 2^12 places them and the sign (the copies of a
+// code do not touch), so eight codes take 11 logic and permute instructions (at half rate) and eight of the multiply pipe; shifts
+// took the logic pipe for 23, byte tables with the scale built in for 15 and 10 per block.  f16 takes the conversion instruction:
+// eight in all.  GEMM of 512 rows x 11008 x 4096: tables bf16 47.3 us, f16 49.2; now 42.2 and 38.2; 16 rows x 14336 x 4096: 21.7 and
+// 22.6; now 19.4 and 16.3.
 template <> struct Mx<__nv_bfloat16> {
-    static constexpr int POS = 6;                        // bit of the code's mantissa bit
-    static constexpr int FAST_MAX = 128;                 // largest byte whose lift is a bf16 number
-    // 2^(byte - 1), twice
-    __device__ static __forceinline__ uint32_t lift(uint32_t b) { return ((b + 126u) << 7) * 0x00010001u; }
-    // the product for any byte: up to 2^127, then the rest
-    __device__ static __forceinline__ uint32_t any(uint32_t field, uint32_t b) {
-        if (b <= FAST_MAX) return P2<__nv_bfloat16>::fma(field, lift(b), 0x80008000u);
-        const uint32_t rest = b == 255u ? 0x7FC0u : (b - 1u) << 7;                       // 2^(b - 128)
-        return P2<__nv_bfloat16>::fma(P2<__nv_bfloat16>::fma(field, lift(128u), 0x80008000u), rest * 0x00010001u, 0x80008000u);
+    static constexpr uint32_t FAST_MIN = 0, FAST_MAX = 128;
+    __device__ static __forceinline__ uint32_t factor(uint32_t b) { return ((b + 126u) << 7) * 0x00010001u; }      // 2^(byte - 1), twice
+    __device__ static __forceinline__ void fields8(uint32_t w, uint32_t (&o)[4]) {
+        const uint32_t even = w & 0x0F0F0F0Fu, odd = w >> 4 & 0x0F0F0F0Fu;
+        o[0] = prmt(even, odd, 0x8480); o[1] = prmt(even, odd, 0x8581);
+        o[2] = prmt(even, odd, 0x8682); o[3] = prmt(even, odd, 0x8783);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * 0x1040u & 0x81C081C0u;
     }
 };
 template <> struct Mx<__half> {
-    static constexpr int POS = 9;
-    static constexpr int FAST_MAX = 128;
-    // 2^(byte - 113), twice; zero below 2^-24, where no weight of the block reaches half of f16's smallest number
-    __device__ static __forceinline__ uint32_t lift(uint32_t b) {
-        const uint32_t h = b >= 99u ? (b - 98u) << 10 : (b >= 89u ? 1u << (b - 89u) : 0u);
-        return h * 0x00010001u;
+    static constexpr uint32_t FAST_MIN = 103, FAST_MAX = 142;                                   // 2^-24 .. 2^15
+    __device__ static __forceinline__ uint32_t factor(uint32_t b) {
+        return (b >= 113u ? (b - 112u) << 10 : 1u << (b - 103u)) * 0x00010001u;                 // 2^(byte - 127), twice
     }
-    __device__ static __forceinline__ uint32_t any(uint32_t field, uint32_t b) {
-        if (b <= FAST_MAX) return P2<__half>::fma(field, lift(b), 0x80008000u);
-        const uint32_t one = P2<__half>::fma(field, lift(128u), 0x80008000u);             // twice the code's value
-        const uint32_t e1 = min(b - 128u, 15u), e2 = min(b - 128u - e1, 15u);             // 2^30 overflows every weight
-        const uint32_t m1 = b == 255u ? 0x7E00u : (e1 + 15u) << 10, m2 = (e2 + 15u) << 10;
-        return P2<__half>::fma(P2<__half>::fma(one, m1 * 0x00010001u, 0x80008000u), m2 * 0x00010001u, 0x80008000u);
-    }
+    __device__ static __forceinline__ void fields8(uint32_t w, uint32_t (&o)[4]) { mx_values8(w, o); }
 };
-
-// The eight magnitudes of a block, scaled, as the byte tables of two byte permutes: a code's three low bits are a permute
-// selector as they stand, so four codes cost a look-up of their high and one of their low bytes, and the scale is
-// multiplied in once per block instead of once per pair.  15 instructions per eight codes and 10 per block; fields shifted
-// into place and multiplied took 23 to the same order.
-template <typename AT> struct MxTable {
-    uint32_t h0, h1, l0, l1;
-    // fast: the byte is at most FAST_MAX (in all lanes of the warp, which branch together)
-    __device__ __forceinline__ void build(uint32_t byte, bool fast) {
-        constexpr uint32_t one = 0x00010001u << Mx<AT>::POS;                 // codes (0, 1), (2, 3), (4, 5), (6, 7) as fields
-        uint32_t t[4];
-        const uint32_t lift = Mx<AT>::lift(byte);
+// the 32 codes of a block; fast: the byte is in the type's range (in all lanes of the warp, which branch together)
+template <typename AT> __device__ __forceinline__ void mx_expand32(const uint32_t (&w)[4], uint32_t byte, bool fast, uint32_t* out) {
+    if (fast) {
+        const uint32_t factor = Mx<AT>::factor(byte);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t f = one * (2u * i) + (0x00010000u << Mx<AT>::POS);
-            t[i] = fast ? P2<AT>::fma(f, lift, 0x80008000u) : Mx<AT>::any(f, byte);
+            uint32_t f[4];
+            Mx<AT>::fields8(w[i], f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[4 * i + j] = P2<AT>::fma(f[j], factor, 0x80008000u);
         }
-        h0 = prmt(t[0], t[1], 0x7531); h1 = prmt(t[2], t[3], 0x7531);
-        l0 = prmt(t[0], t[1], 0x6420); l1 = prmt(t[2], t[3], 0x6420);
+    } else {
+        const float scale = mx_scale_f32(byte);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t f[4];
+            mx_values8(w[i], f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                out[4 * i + j] = Act<AT>::pack_hi(Act<__half>::lo_f32(f[j]) * scale, Act<__half>::hi_f32(f[j]) * scale);
+        }
     }
-    // eight codes -> four pairs in order
-    __device__ __forceinline__ void expand(uint32_t w, uint32_t* o) const {
-        const uint32_t s = w & 0x77777777u, s2 = s >> 16, up = w << 4;
-        // sign bytes: bit 3 of a code is the top bit of its byte in w (odd codes) or w << 4 (even ones)
-        const uint32_t a = and_or(prmt(up, w, 0xD9C8), 0x80808080u, prmt(h0, h1, s)), la = prmt(l0, l1, s);
-        const uint32_t b = and_or(prmt(up, w, 0xFBEA), 0x80808080u, prmt(h0, h1, s2)), lb = prmt(l0, l1, s2);
-        o[0] = prmt(la, a, 0x5140); o[1] = prmt(la, a, 0x7362);
-        o[2] = prmt(lb, b, 0x5140); o[3] = prmt(lb, b, 0x7362);
-    }
-};
+}
 
 }  // namespace jq

@@ -82,14 +82,6 @@ __device__ __forceinline__ void mx_scales4(uint32_t w, bool fast, float (&f)[4])
         f[0] = mx_scale_any<0>(w); f[1] = mx_scale_any<1>(w); f[2] = mx_scale_any<2>(w); f[3] = mx_scale_any<3>(w);
     }
 }
-// eight codes -> four f16 pairs of their plain values, in order
-__device__ __forceinline__ void mx_values8(uint32_t w, uint32_t (&o)[4]) {
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-        : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
-        : "r"(w));
-}
-
 // One activation row into shared memory as f16, zeros from K to the end of its last stretch.  bf16: block b is multiplied by
 // 2^-e and scales[b * stride] = 2^e, e such that the block's largest is in [2^14, 2^15) (not below 2^-100: smaller blocks lose
 // bits below 2^-125).  A block with an infinity or a NaN keeps those as they are and nothing else: the products are the same.

@@ -162,15 +162,13 @@ __device__ __forceinline__ void expand_block_mx(const uint8_t* crow, int r, int 
         sb = sc.ns;
         if (kb_next >= 0) sc.fetch(kb_next);
     }
-    const bool fast = __all_sync(0xFFFFFFFFu, max(sb & 255u, sb >> 8) <= (uint32_t)Mx<AT>::FAST_MAX);
+    const uint32_t b0 = sb & 255u, b1 = sb >> 8;
+    const bool fast = __all_sync(0xFFFFFFFFu, max(b0, b1) <= Mx<AT>::FAST_MAX && (Mx<AT>::FAST_MIN == 0u || min(b0, b1) >= Mx<AT>::FAST_MIN));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint4 v = cp[code_chunk<CPR>(kbi * 2 + h, r)];
         const uint32_t cur[4] = {v.x, v.y, v.z, v.w};
-        MxTable<AT> table;
-        table.build(h ? sb >> 8 : sb & 255u, fast);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) table.expand(cur[i], out + 16 * h + 4 * i);
+        mx_expand32<AT>(cur, h ? b1 : b0, fast, out + 16 * h);
     }
 }
 

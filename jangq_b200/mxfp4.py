@@ -18,8 +18,9 @@ from ._lib import JangqError
 BLOCK = 32
 SORT_THRESHOLD = 64      # pairs; as gather_qmm
 # Rows that the mat-vec takes in one launch (their activations in shared memory: rows * K up to MXFP4_GEMV_MAX_K).  Beyond,
-# every weight is read again, and the tensor-core GEMM is faster: 8 rows of 14336x4096 16.7 us here, 22.2 there, 9 rows 29 and
-# 22; 8 rows of 2048x2048 5.8 and 6.6, 9 rows 10 and 6.7; 2 rows of 4096x14336 15.2 and 20.7, 4 rows 29 and 21.
+# every weight is read again, and the tensor-core GEMM is faster: bf16, 8 rows of 14336x4096 16.8 us here, 20.4 there, 9 rows 29
+# and 20; 8 rows of 4096x4096 9.5 and 9.3, of 2048x2048 5.8 and 6.3, 9 rows 10 and 6.4; 2 rows of 4096x14336 15.3 and 19.0, 4 rows
+# 29 and 19; f16, 8 rows of 14336x4096 14.1 and 17.3.
 MATVEC_ROWS = 8
 
 
