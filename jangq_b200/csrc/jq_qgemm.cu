@@ -42,6 +42,7 @@ namespace jq {
 
 constexpr int GEMM_BM = 128;
 constexpr int GEMM_BK = 64;
+constexpr int GEMM_BOX_HIGH = 128, GEMM_BOX_LOW = 32;      // activation rows per TMA box in grouped mode
 constexpr int GEMM_SMEM = 227 * 1024;   // dynamic shared memory of one CTA
 
 struct GemmArgs {
@@ -52,7 +53,7 @@ struct GemmArgs {
     int64_t M, N, K, ldy;
     int gs, G;
     int tn;          // activation rows per tile (multiple of 16, <= TNMAX)
-    int box_rows;    // activation rows per TMA box: tn, or 32 when the rows of a tile vary (grouped mode)
+    int box_rows;    // activation rows per TMA box: tn, or, when the rows of a tile vary (grouped mode), of the high one
     int y_pair_ok;   // rows of y are 4-byte aligned
     int y_vec_ok;    // rows of y are 8-byte aligned
     int* status;     // device status word, set to 1 when a bounded wait ran out
@@ -541,7 +542,7 @@ template <bool GU> __device__ __forceinline__ int pers_side_mode(const GemmArgs&
 
 template <typename AT, int BITS, bool GU, int TN, bool MX = false, bool SC = false>
 __global__ void __launch_bounds__(PersCfg<BITS, TN>::THREADS, 1)
-qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
+qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap xmap_low, const GemmArgs a) {
     using C = PersCfg<BITS, TN>;
     constexpr int CKB = C::CKB, RB = C::RB, CD = C::CD, RA = C::RA, NKG = C::NKG;
 
@@ -587,27 +588,34 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
     };
 
     if (warp == 0) {
-        // ---------------- TMA producer ----------------
-        int s = 0;
-        uint32_t ph = 1u;
-        for (int tile = first; tile < total && ok; tile += step) {
-            const PersTile t = take(tile);
-            if (t.rows <= 0) continue;
-            const int boxes = (((t.rows + 15) & ~15) + a.box_rows - 1) / a.box_rows;
-            const uint32_t box_bytes = (uint32_t)(a.box_rows * GEMM_BK * 2), bytes = (uint32_t)boxes * box_bytes;
-            for (int i = 0; i < nkb; ++i) {
-                ok = __all_sync(0xFFFFFFFFu, ts_wait(empty + s, ph));
-                if (!ok) break;
-                if (elect_one()) {
+        // ---------------- TMA producer: one thread ----------------
+        // A copy instruction takes its thread some 80 cycles, so a tile is covered with few: boxes of 128 rows, and for up to 64
+        // that are left boxes of 32 (with 32 alone the five copies of a tile of 130 rows took 650 cycles, the pace of the k-loop:
+        // 16384 rows over 128 experts of 768 x 2048 BOX_BEFORE us, now BOX_AFTER).
+        if (elect_one()) {
+            int s = 0;
+            uint32_t ph = 1u;
+            for (int tile = first; tile < total && ok; tile += step) {
+                const PersTile t = take(tile);
+                if (t.rows <= 0) continue;
+                const int high = (t.rows + GEMM_BOX_HIGH - 1 - 2 * GEMM_BOX_LOW) / GEMM_BOX_HIGH;
+                const int low = (max(t.rows - high * GEMM_BOX_HIGH, 0) + GEMM_BOX_LOW - 1) / GEMM_BOX_LOW;
+                const uint32_t bytes = (uint32_t)((high * GEMM_BOX_HIGH + low * GEMM_BOX_LOW) * GEMM_BK * 2);
+                for (int i = 0; i < nkb; ++i) {
+                    ok = ts_wait(empty + s, ph);
+                    if (!ok) break;
                     mbar_expect_tx(full + s, bytes);
-                    for (int b = 0; b < boxes; ++b)          // rows past M read as zeros
-                        tma_load_2d(sX + s * C::X_STAGE + b * box_bytes, &xmap, i * GEMM_BK, (int)t.m0 + b * a.box_rows,
-                                    full + s);
+                    uint8_t* dst = sX + s * C::X_STAGE;          // rows past M read as zeros
+                    int row = (int)t.m0;
+                    for (int b = 0; b < high; ++b, row += GEMM_BOX_HIGH, dst += GEMM_BOX_HIGH * GEMM_BK * 2)
+                        tma_load_2d(dst, &xmap, i * GEMM_BK, row, full + s);
+                    for (int b = 0; b < low; ++b, row += GEMM_BOX_LOW, dst += GEMM_BOX_LOW * GEMM_BK * 2)
+                        tma_load_2d(dst, &xmap_low, i * GEMM_BK, row, full + s);
+                    if (++s == RA) { s = 0; ph ^= 1u; }
                 }
-                __syncwarp();
-                if (++s == RA) { s = 0; ph ^= 1u; }
             }
         }
+        ok = __all_sync(0xFFFFFFFFu, ok);
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         const uint32_t x_lo = umma_desc_sw128_lo(smem_u32(sX));
@@ -832,7 +840,7 @@ static int launch_gemm(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_til
 }
 
 template <typename AT, int BITS, bool GU, int TN, bool MX = false, bool SC = false>
-static int launch_pers(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_tiles, cudaStream_t st) {
+static int launch_pers(const CUtensorMap& xmap, const CUtensorMap& xmap_low, const GemmArgs& a, int64_t m_tiles, cudaStream_t st) {
     using C = PersCfg<BITS, TN>;
     static_assert(C::SMEM <= GEMM_SMEM, "shared memory of one CTA");
     auto kernel = qgemm_pers_kernel<AT, BITS, GU, TN, MX, SC>;
@@ -846,7 +854,7 @@ static int launch_pers(const CUtensorMap& xmap, const GemmArgs& a, int64_t m_til
     const int64_t nx = (a.N + (GU ? 63 : 127)) / (GU ? 64 : 128), tiles = nx * m_tiles;
     JQ_REQUIRE(tiles < (1ll << 31), JQ_EUNSUPPORTED, "too many tiles for one launch (%lld)", (long long)tiles);
     const unsigned grid = (unsigned)std::min<int64_t>(tiles, sm_count());
-    kernel<<<grid, C::THREADS, C::SMEM, st>>>(xmap, a);
+    kernel<<<grid, C::THREADS, C::SMEM, st>>>(xmap, xmap_low, a);
     return check_launch("qgemm");
 }
 
@@ -924,7 +932,7 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
         JQ_REQUIRE(grp->tile_m == 128 || grp->tile_m == 192 || (grp->tile_m == 256 && N >= 256 && x_dtype == JQ_BF16),
                    JQ_EUNSUPPORTED, "tile lists of 256 rows need bf16 activations and N >= 256 (128 or 192 otherwise)");
         a.tn = grp->tile_m;
-        a.box_rows = 32;
+        a.box_rows = GEMM_BOX_HIGH;
         m_tiles = grp->max_tiles;
     } else {
         // The number of row tiles (nt, of tn rows each) and the K split with the shortest estimated time.  Measured on
@@ -953,30 +961,33 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
     if (m_tiles == 0) return JQ_OK;
     JQ_REQUIRE((grp ? grp->max_tiles : (M + GEMM_BM - 1) / GEMM_BM) < 65536, JQ_EUNSUPPORTED,
                "too many row tiles for one launch (%lld)", (long long)(grp ? grp->max_tiles : (M + GEMM_BM - 1) / GEMM_BM));
-    CUtensorMap xmap;
+    CUtensorMap xmap, xmap_low;
     const cuuint64_t gdim[2] = {(cuuint64_t)K, (cuuint64_t)M};
     const cuuint64_t gstride[1] = {(cuuint64_t)ldx * 2};
-    const cuuint32_t box[2] = {GEMM_BK, (cuuint32_t)a.box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    CUresult cr = enc(&xmap, x_dtype == JQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                      const_cast<void*>(x), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    JQ_REQUIRE(cr == CUDA_SUCCESS, JQ_ECUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
+    for (CUtensorMap* map : {&xmap, &xmap_low}) {
+        if (map == &xmap_low && !grp) break;
+        const cuuint32_t box[2] = {GEMM_BK, (cuuint32_t)(map == &xmap ? a.box_rows : GEMM_BOX_LOW)};
+        CUresult cr = enc(map, x_dtype == JQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                          const_cast<void*>(x), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        JQ_REQUIRE(cr == CUDA_SUCCESS, JQ_ECUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
+    }
 
 #define JQ_GEMM_T(T, B)                                                                                   \
     {                                                                                                     \
-        if (gu) return launch_pers<T, B, true, 192>(xmap, a, m_tiles, st);                                \
-        if (grp) return launch_pers<T, B, false, 192>(xmap, a, m_tiles, st);                              \
+        if (gu) return launch_pers<T, B, true, 192>(xmap, xmap_low, a, m_tiles, st);                      \
+        if (grp) return launch_pers<T, B, false, 192>(xmap, xmap_low, a, m_tiles, st);                    \
         if (ks == 4) return launch_gemm<T, B, 4>(xmap, a, m_tiles, st);                                   \
         if (ks == 2) return launch_gemm<T, B, 2>(xmap, a, m_tiles, st);                                   \
         return launch_gemm<T, B, 1>(xmap, a, m_tiles, st);                                                \
     }
 #define JQ_GEMM_MX(T)                                                                                     \
     {                                                                                                     \
-        if (gu) return launch_pers<T, 4, true, 192, true>(xmap, a, m_tiles, st);                          \
-        if (sc) return launch_pers<T, 4, false, 192, true, true>(xmap, a, m_tiles, st);                   \
-        if (grp) return launch_pers<T, 4, false, 192, true>(xmap, a, m_tiles, st);                        \
+        if (gu) return launch_pers<T, 4, true, 192, true>(xmap, xmap_low, a, m_tiles, st);                \
+        if (sc) return launch_pers<T, 4, false, 192, true, true>(xmap, xmap_low, a, m_tiles, st);         \
+        if (grp) return launch_pers<T, 4, false, 192, true>(xmap, xmap_low, a, m_tiles, st);              \
         if (ks == 4) return launch_gemm<T, 4, 4, true>(xmap, a, m_tiles, st);                             \
         if (ks == 2) return launch_gemm<T, 4, 2, true>(xmap, a, m_tiles, st);                             \
         return launch_gemm<T, 4, 1, true>(xmap, a, m_tiles, st);                                          \
@@ -988,8 +999,8 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
 #define JQ_GEMM_CASE(B)                                                                                   \
     if (bits == B) {                                                                                      \
         if (grp && grp->tile_m == 256)                         /* bf16 only, see above */                 \
-            return gu ? launch_pers<__nv_bfloat16, B, true, 256>(xmap, a, m_tiles, st)                    \
-                      : launch_pers<__nv_bfloat16, B, false, 256>(xmap, a, m_tiles, st);                  \
+            return gu ? launch_pers<__nv_bfloat16, B, true, 256>(xmap, xmap_low, a, m_tiles, st)          \
+                      : launch_pers<__nv_bfloat16, B, false, 256>(xmap, xmap_low, a, m_tiles, st);        \
         if (x_dtype == JQ_BF16) JQ_GEMM_T(__nv_bfloat16, B)                                               \
         JQ_GEMM_T(__half, B)                                                                              \
     }
