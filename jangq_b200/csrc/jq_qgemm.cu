@@ -56,6 +56,7 @@ struct GemmArgs {
     int box_rows;    // activation rows per TMA box: tn, or, when the rows of a tile vary (grouped mode), of the high one
     int y_pair_ok;   // rows of y are 4-byte aligned
     int y_vec_ok;    // rows of y are 8-byte aligned
+    int y_vec16_ok;  // ... 16-byte aligned
     int* status;     // device status word, set to 1 when a bounded wait ran out
     // grouped mode (routed experts): CTAs walk a tile list built by jq_moe_sort; rows are the expert-sorted
     // (token, slot) pairs, weights come from per-expert pointer tables
@@ -198,22 +199,23 @@ __device__ __forceinline__ void store_columns(const GemmArgs& a, const uint32_t 
     }
 }
 
-// the same, to the rows that the lanes hold: lane j's `to` is the row of y of column j
+// The same, to the rows that the lanes hold: lane j's `to` is the row of y of column j.  Whole rows of 16-byte vectors go through
+// the warp's 2 KB of shared memory, 64 bytes of a row per four lanes.
 template <typename AT>
 __device__ __forceinline__ void scatter_columns(const GemmArgs& a, const uint32_t (&v)[32], int to, int rows, int64_t nn, bool whole,
-                                                int lane) {
+                                                int lane, uint16_t* sw) {
     using A = Act<AT>;
     uint16_t* yb = reinterpret_cast<uint16_t*>(a.y);
-    if (a.y_pair_ok && whole) {
-        const int odd = lane & 1;
-        uint16_t* yl = yb + (nn & ~1ll);
+    if (a.y_vec16_ok && whole) {
+        __syncwarp();                                          // the columns before have been read
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            const float keep = __uint_as_float(odd ? v[j + 1] : v[j]);
-            const float got = __uint_as_float(__shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1));
-            const int row = __shfl_sync(0xFFFFFFFFu, to, j + odd);
-            const uint32_t pk = odd ? A::pack_hi(got, keep) : A::pack_hi(keep, got);
-            if (j + odd < rows) *reinterpret_cast<uint32_t*>(yl + row * a.ldy) = pk;
+        for (int j = 0; j < 32; ++j) sw[j * 32 + lane] = A::from_f32(__uint_as_float(v[j]));
+        __syncwarp();
+        const int64_t col = (nn & ~31ll) + (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = 8 * i + (lane >> 2), row = __shfl_sync(0xFFFFFFFFu, to, j);
+            if (j < rows) *reinterpret_cast<uint4*>(yb + row * a.ldy + col) = reinterpret_cast<const uint4*>(sw)[i * 32 + lane];
         }
     } else {
 #pragma unroll
@@ -503,7 +505,7 @@ template <int BITS, int TN> struct PersCfg {
     static constexpr int NDW = 4 * NKG, THREADS = 32 * (8 + NDW);
     static constexpr int NBAR = 2 * RA + 2 * CD + 2 * ND;
     static constexpr int SIDE_OFF = RA * X_STAGE + CD * C_STAGE;
-    static constexpr int SW_OFF = SIDE_OFF + CD * SIDE_SLOT;             // float[32][128]: gate/up exchange
+    static constexpr int SW_OFF = SIDE_OFF + CD * SIDE_SLOT;             // float[32][128]: gate/up exchange; scatter mode: [4][32][32]
     static constexpr int WT_OFF = SW_OFF + 32 * 128 * 4;                 // float[TN]: routing weights of the tile's rows
     static constexpr int BAR_OFF = WT_OFF + TNMAX * 4;
     static constexpr size_t SMEM = 1024 + BAR_OFF + NBAR * 8 + 16;
@@ -716,7 +718,8 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
                     int here = to[0];
 #pragma unroll
                     for (int i = 1; i < C::TNMAX / 32; ++i) here = c0 == i * 32 ? to[i] : here;
-                    scatter_columns<AT>(a, v, here, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane);
+                    scatter_columns<AT>(a, v, here, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane,
+                                        reinterpret_cast<uint16_t*>(smem + C::SW_OFF) + quarter * 1024);
                 } else {
                     store_columns<AT>(a, v, t.m0 + c0, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane);
                 }
@@ -907,6 +910,7 @@ int qgemm_dispatch(const void* x, int x_dtype, int64_t M, int64_t ldx, const uin
     a.M = M; a.N = N; a.K = K; a.ldy = ldy; a.gs = gs; a.G = (int)(K / gs);
     a.y_pair_ok = (aligned(y, 4) && ldy % 2 == 0) ? 1 : 0;
     a.y_vec_ok = (aligned(y, 8) && ldy % 4 == 0) ? 1 : 0;
+    a.y_vec16_ok = (aligned(y, 16) && ldy % 8 == 0) ? 1 : 0;
     a.status = status_word();
     JQ_REQUIRE(a.status != nullptr, JQ_ECUDA, "could not locate the device status word");
     a.tile_expert = grp ? grp->tile_expert : nullptr;
