@@ -174,13 +174,32 @@ __device__ __forceinline__ void expand_block_mx(const uint8_t* crow, int r, int 
     }
 }
 
+// 32 accumulator columns of one weight row per lane to the rows row(j) of y, `rows` of them, through the warp's 2 KB of shared
+// memory: four lanes store 64 bytes of a row.  (With 4 bytes per lane, straight from the registers, the epilogue of a 128-row
+// tile took 7000 cycles on its own and 12500 beside the k-loop; 8192 rows over 32 experts of 640 x 1152 35 us, now 28.)
+template <typename AT, typename Row>
+__device__ __forceinline__ void store_rows16(const GemmArgs& a, const uint32_t (&v)[32], int rows, int64_t nn, int lane, uint16_t* sw, Row row) {
+    __syncwarp();                                              // the columns before have been read
+#pragma unroll
+    for (int j = 0; j < 32; ++j) sw[j * 32 + lane] = Act<AT>::from_f32(__uint_as_float(v[j]));
+    __syncwarp();
+    uint16_t* yl = reinterpret_cast<uint16_t*>(a.y) + (nn & ~31ll) + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = 8 * i + (lane >> 2);
+        const int64_t to = row(j);
+        if (j < rows) *reinterpret_cast<uint4*>(yl + to * a.ldy) = reinterpret_cast<const uint4*>(sw)[i * 32 + lane];
+    }
+}
 // 32 accumulator columns (activation rows row0 .. row0 + 31 of y, `rows` of them valid) of one weight row per lane
 template <typename AT>
 __device__ __forceinline__ void store_columns(const GemmArgs& a, const uint32_t (&v)[32], int64_t row0, int rows, int64_t nn,
-                                              bool whole, int lane) {
+                                              bool whole, int lane, uint16_t* sw) {
     using A = Act<AT>;
     uint16_t* yb = reinterpret_cast<uint16_t*>(a.y) + row0 * a.ldy;
-    if (a.y_pair_ok && whole) {
+    if (a.y_vec16_ok && whole) {
+        store_rows16<AT>(a, v, rows, nn, lane, sw, [&](int j) { return row0 + j; });
+    } else if (a.y_pair_ok && whole) {
         // neighbouring lanes swap halves: an even lane stores rows (n, n+1) of the even columns, an
         // odd lane (n-1, n) of the odd ones, 4 bytes each
         const bool odd = lane & 1;
@@ -199,24 +218,14 @@ __device__ __forceinline__ void store_columns(const GemmArgs& a, const uint32_t 
     }
 }
 
-// The same, to the rows that the lanes hold: lane j's `to` is the row of y of column j.  Whole rows of 16-byte vectors go through
-// the warp's 2 KB of shared memory, 64 bytes of a row per four lanes.
+// the same, to the rows that the lanes hold: lane j's `to` is the row of y of column j
 template <typename AT>
 __device__ __forceinline__ void scatter_columns(const GemmArgs& a, const uint32_t (&v)[32], int to, int rows, int64_t nn, bool whole,
                                                 int lane, uint16_t* sw) {
     using A = Act<AT>;
     uint16_t* yb = reinterpret_cast<uint16_t*>(a.y);
     if (a.y_vec16_ok && whole) {
-        __syncwarp();                                          // the columns before have been read
-#pragma unroll
-        for (int j = 0; j < 32; ++j) sw[j * 32 + lane] = A::from_f32(__uint_as_float(v[j]));
-        __syncwarp();
-        const int64_t col = (nn & ~31ll) + (lane & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = 8 * i + (lane >> 2), row = __shfl_sync(0xFFFFFFFFu, to, j);
-            if (j < rows) *reinterpret_cast<uint4*>(yb + row * a.ldy + col) = reinterpret_cast<const uint4*>(sw)[i * 32 + lane];
-        }
+        store_rows16<AT>(a, v, rows, nn, lane, sw, [&](int j) { return (int64_t)__shfl_sync(0xFFFFFFFFu, to, j); });
     } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
@@ -438,7 +447,8 @@ qgemm_ts_kernel(const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
                     for (int j = 0; j < 32; ++j)
                         if (c0 + j < rows) part[j * 128] = __uint_as_float(v[j]);
                 } else {
-                    store_columns<AT>(a, v, m0 + c0, rows - c0, nn, n0 + 128 <= a.N, lane);
+                    store_columns<AT>(a, v, m0 + c0, rows - c0, nn, n0 + 128 <= a.N, lane,
+                                      reinterpret_cast<uint16_t*>(smem) + (warp - 4) * 1024);       // activation stages, idle now
                 }
             }
         }
@@ -505,7 +515,7 @@ template <int BITS, int TN> struct PersCfg {
     static constexpr int NDW = 4 * NKG, THREADS = 32 * (8 + NDW);
     static constexpr int NBAR = 2 * RA + 2 * CD + 2 * ND;
     static constexpr int SIDE_OFF = RA * X_STAGE + CD * C_STAGE;
-    static constexpr int SW_OFF = SIDE_OFF + CD * SIDE_SLOT;             // float[32][128]: gate/up exchange; scatter mode: [4][32][32]
+    static constexpr int SW_OFF = SIDE_OFF + CD * SIDE_SLOT;             // float[32][128]: gate/up exchange; else a warp's [32][32] results
     static constexpr int WT_OFF = SW_OFF + 32 * 128 * 4;                 // float[TN]: routing weights of the tile's rows
     static constexpr int BAR_OFF = WT_OFF + TNMAX * 4;
     static constexpr size_t SMEM = 1024 + BAR_OFF + NBAR * 8 + 16;
@@ -721,7 +731,8 @@ qgemm_pers_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
                     scatter_columns<AT>(a, v, here, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane,
                                         reinterpret_cast<uint16_t*>(smem + C::SW_OFF) + quarter * 1024);
                 } else {
-                    store_columns<AT>(a, v, t.m0 + c0, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane);
+                    store_columns<AT>(a, v, t.m0 + c0, t.rows - c0, t.n0 + r, t.n0 + 128 <= a.N, lane,
+                                      reinterpret_cast<uint16_t*>(smem + C::SW_OFF) + quarter * 1024);
                 }
             }
             if (++d == C::ND) { d = 0; dph ^= 1u; }
