@@ -26,7 +26,7 @@ struct Gemm4Args {
     int tn;                  // activation rows per tile, a multiple of 16
     int mt, tiles;           // CTA pairs: tiles along M, and in all (activation rows vary fastest)
     int vec;                 // every row's scales are whole 16-byte vectors
-    int y_pair_ok;
+    int y_pair_ok, y_vec_ok;         // rows of y are 4-byte, 16-byte aligned
     int* status;
 };
 
@@ -314,6 +314,11 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
                 f.x += o.x; f.y += o.y; f.z += o.z; f.w += o.w;
             }
             OT* yp = reinterpret_cast<OT*>(a.y) + (m0 + tok) * a.ldy + n0 + nl;
+            if (a.y_vec_ok && n0 + nl + 4 <= a.N) {
+                if constexpr (sizeof(OT) == 4) *reinterpret_cast<float4*>(yp) = f;
+                else *reinterpret_cast<uint2*>(yp) = make_uint2(Act<OT>::pack_hi(f.x, f.y), Act<OT>::pack_hi(f.z, f.w));
+                continue;
+            }
             const float fv[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -337,7 +342,7 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
 // ---- more rows: CTA pairs walk tiles of 256 weight rows x up to 256 activation rows ---------------------------
 // Each CTA copies its 128 weight rows and half of the activation rows; the MMAs of the first CTA (cta_group::2) read both
 // halves from both CTAs' shared memory, so a code byte is copied from L2 half as often as with one CTA per tile -- those
-// copies are the bound: tiles of 224 rows with two whole accumulators were slower (115 us for 4096 rows x 14336 x 4096).
+// copies are the bound: tiles of 224 rows with two whole accumulators were slower (115 us for 4096 rows x 14336 x 4096; this form 96 to 98 = 4.9 PFLOP/s, 12.8 TB/s out of L2).
 // Tensor memory holds two accumulators of 256 columns that share 48: the epilogue warps read those first, and the next
 // tile's MMAs run into the other one while they take and store the rest (with a single accumulator the MMAs stood still for
 // 1.7 of 7.4 us per tile).  The remaining 48 columns are the scales of two stages: a stage's are copied once the MMAs of the
@@ -347,7 +352,8 @@ mxfp4_gemm4_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
 //   accempty   in the first CTA, once per tile: the epilogue warps of both have read the tile before and the shared columns
 constexpr int G4P_RA = 5, G4P_TN = 256, G4P_SF = 3 * 1024, G4P_THREADS = 512, G4P_SFCOLS = 24, G4P_EPI = 8;
 constexpr int G4P_SETS = 2, G4P_SLOTS = 2 * G4P_SETS, G4P_SHARE = 48, G4P_D1 = G4P_TN - G4P_SHARE, G4P_DCOLS = G4P_D1 + G4P_TN;
-constexpr size_t G4P_SMEM = 1024 + (size_t)G4P_RA * 2 * G4_A + G4P_SLOTS * G4_GS * G4P_SF + (2 * G4P_RA + 2 * G4P_SLOTS + 3) * 8 + 16;
+constexpr int G4P_STORE = G4P_RA * 2 * G4_A + G4P_SLOTS * G4_GS * G4P_SF;          // 2 KB per epilogue warp
+constexpr size_t G4P_SMEM = 1024 + (size_t)G4P_STORE + G4P_EPI * 2048 + (2 * G4P_RA + 2 * G4P_SLOTS + 3) * 8 + 16;
 static_assert(G4P_SMEM <= 227 * 1024, "shared memory of one CTA");
 static_assert(G4P_DCOLS + 2 * G4P_SFCOLS <= G4_NCOLS, "tensor memory");
 
@@ -403,7 +409,7 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sA = smem, *sB = sA + G4P_RA * G4_A, *sS = sB + G4P_RA * G4_A;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sS + G4P_SLOTS * G4_GS * G4P_SF);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + G4P_STORE + G4P_EPI * 2048);
     uint64_t* empty = full + G4P_RA;
     uint64_t* sfull = empty + G4P_RA;
     uint64_t* sempty = sfull + G4P_SLOTS;
@@ -542,9 +548,9 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
             const uint32_t src = src0 + d * G4P_D1;
             bool stored = false;
             if constexpr (sizeof(OT) == 2) {
-                if (a.y_pair_ok && n0 + 128 <= a.N) {
+                if (a.y_vec_ok && n0 + 128 <= a.N) {
                     // rounded to pairs of neighbouring activation rows, the columns that the other accumulator shares first
-                    // (the last 48 of the first accumulator, the first 48 of the second), then stored as in store_tile32
+                    // (the last 48 of the first accumulator, the first 48 of the second)
                     uint32_t pk[COLS / 2];
                     auto take = [&](int c) {
                         uint32_t v[16];
@@ -576,13 +582,24 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
                         for (int c = 0; c < COLS / 16; ++c) take(c);
                     }
                     stored = true;
-                    const int odd = lane & 1;
-                    OT* yl = y + (odd ? a.ldy : 0) + (nn & ~1ll);
+                    // 32 activation rows at a time through the warp's 2 KB: four lanes store 64 bytes of a row (4 bytes per lane,
+                    // straight from the registers: 1024 rows x 4096 x 4096 16.1 us, now 14.3)
+                    uint16_t* sw = reinterpret_cast<uint16_t*>(smem + G4P_STORE) + (warp - 8) * 1024;
+                    OT* yl = y + (nn & ~31ll) + (lane & 3) * 8;
 #pragma unroll
-                    for (int j = 0; j < COLS / 2; ++j) {
-                        const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, pk[j], 1);
-                        const uint32_t out = odd ? prmt(other, pk[j], 0x7632) : prmt(pk[j], other, 0x5410);
-                        if (2 * j + odd < rows) *reinterpret_cast<uint32_t*>(yl + 2 * j * a.ldy) = out;
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            sw[2 * j * 32 + lane] = (uint16_t)pk[c * 16 + j];
+                            sw[(2 * j + 1) * 32 + lane] = (uint16_t)(pk[c * 16 + j] >> 16);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = c * 32 + 8 * i + (lane >> 2);
+                            if (j < rows) *reinterpret_cast<uint4*>(yl + j * a.ldy) = reinterpret_cast<const uint4*>(sw)[i * 32 + lane];
+                        }
                     }
                 }
             }
@@ -620,11 +637,11 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
 }
 
 // What the choice of a form goes by (us on B200; K stages of 256 codes).  One CTA per tile: 2 once, then per wave of tiles 2.2 and
-// 0.205 + 0.00085 tn per stage; a split of K adds 0.7 + 0.011 tn.  CTA pairs: 8.7 once, then 0.04 + 0.0015 tn per stage and round.
-// Measured: 16 rows 4096x4096 7.6 unsplit, 6.5 by 2, 6.0 by 4, 13.1 in pairs; 128 rows 2048x8192 12.7, 11.0, 9.0, 19.7; 256 rows
-// 4096x4096 9.0, 9.0, 15.4, 15.6; 1024 rows 4096x4096 16.0, 30.6, 53.5, 16.0; 4096 rows 14336x4096 181 unsplit, 97.5 in pairs.
+// 0.205 + 0.00085 tn per stage; a split of K adds 0.7 + 0.011 tn.  CTA pairs: 7.2 once, then 0.04 + 0.0015 tn per stage and round.
+// Measured: 16 rows 4096x4096 7.6 unsplit, 6.5 by 2, 6.0 by 4, 10.2 in pairs; 128 rows 2048x8192 12.7, 11.0, 9.0, 15.4; 256 rows
+// 4096x4096 9.0, 9.0, 15.4, 12.3; 1024 rows 4096x4096 16.0, 30.6, 53.5, 14.3; 4096 rows 14336x4096 181 unsplit, 96 to 98 in pairs.
 constexpr double G4_T_ONCE = 2.0, G4_T_WAVE = 2.2, G4_T_STAGE = 0.205, G4_T_ROW = 0.00085, G4_T_SPLIT = 0.7, G4_T_SPLIT_ROW = 0.011;
-constexpr double G4_T_PAIR = 8.7, G4_T_PSTAGE = 0.04, G4_T_PROW = 0.0015;
+constexpr double G4_T_PAIR = 7.2, G4_T_PSTAGE = 0.04, G4_T_PROW = 0.0015;
 
 static int encode_codes(CUtensorMap* map, const void* codes, int64_t rows, int64_t K, int box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();
@@ -723,6 +740,7 @@ extern "C" int jq_mxfp4_gemm4(const uint32_t* xcodes, const uint8_t* xscales, in
     a.tiles = (int)pair_tiles;
     a.vec = a.nblk % 16 == 0 && aligned(wscales, 16) && aligned(xscales, 16);
     a.y_pair_ok = (aligned(y, 4) && ldy % 2 == 0) ? 1 : 0;
+    a.y_vec_ok = (aligned(y, 16) && ldy % 8 == 0) ? 1 : 0;
     a.status = status_word();
     JQ_REQUIRE(a.status != nullptr, JQ_ECUDA, "could not locate the device status word");
     CUtensorMap wmap, xmap;
