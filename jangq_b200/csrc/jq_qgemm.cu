@@ -16,13 +16,15 @@
 //                 biases, six stages deep, completion counted on mbarriers (no barrier between warps);
 //   dequantizers  four groups of four warps, one weight row per thread: group g takes k-blocks g, g + 4, ... and owns
 //                 A slot g.
+// MXFP4 weights take the same path with their own expansion (expand_block_mx); their two scale bytes per k-block travel as a
+// 16-bit sidecar.
 // Two forms: one tile per CTA with an optional split of K over a cluster (dense products), and a persistent one that
 // walks the tiles of the routed experts.
 // Every mbarrier wait is bounded; a wait that runs out sets the library's status word and the
 // CTA leaves through the common exit (tensor memory is always released).
 //
-// Measured (B200, N x K): 4096 rows, 14336x4096 4-bit 492 -> 364 us (978 -> 1322 TFLOP/s); 512 rows, 11008x4096 2-bit
-// 68 -> 50 us; 333 rows, 4096x4096 8-bit f16 55 -> 20 us; 61 rows, 4096x4096 6-bit 34 -> 12 us (before: the dequantized
+// Measured (B200, N x K): 4096 rows, 14336x4096 4-bit 492 -> 354 us (978 -> 1360 TFLOP/s); 512 rows, 11008x4096 2-bit
+// 68 -> 40 us; 333 rows, 4096x4096 8-bit f16 55 -> 20 us; 61 rows, 4096x4096 6-bit 34 -> 12 us (before: the dequantized
 // tile as the B operand in shared memory, one thread per weight row, one group of dequantizer warps).
 //
 // Numerics: the A operand is the dequantized weight rounded once to the activation type (what
