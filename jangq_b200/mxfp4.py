@@ -147,9 +147,9 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
 
 class MXFP4ExpertBank:
     """MXFP4 weights of E experts for one projection: `weight` int32/uint32 [E, N, K/8], `scales` uint8 [E, N, K/32].
-    Device pointer tables for the grouped products are built once."""
+    Device pointer tables for the grouped products are built once (one_call: for use on the stream that is current now)."""
 
-    def __init__(self, weight: torch.Tensor, scales: torch.Tensor):
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, one_call: bool = False):
         self.device = _lib.require_cuda(weight, scales)
         if weight.dim() != 3:
             raise JangqError(_lib.JQ_EINVAL, f"stacked expert weight must be [E, N, K/8], got {tuple(weight.shape)}")
@@ -158,9 +158,13 @@ class MXFP4ExpertBank:
         wstep, sstep = self.N * self.K // 2, self.N * self.K // BLOCK
         if self.E < 1 or self.N < 1:
             raise JangqError(_lib.JQ_EINVAL, f"a bank holds at least one row of one expert, got {tuple(weight.shape)}")
-        experts = torch.arange(self.E, dtype=torch.int64, device=self.device)
-        self.codes_tab = self.weight.data_ptr() + experts * wstep
-        self.scales_tab = self.scales.data_ptr() + experts * sstep
+        # The pointers are complete when the constructor returns: a product on another stream that does not wait for this one would
+        # read wrong numbers from weights on their way, but fault on pointers.  A capture (and a bank of one call, whose products
+        # follow on the same stream) cannot wait.
+        wait = not (one_call or torch.cuda.is_current_stream_capturing())
+        experts = torch.arange(self.E, dtype=torch.int64, device="cpu" if wait else self.device)
+        self.codes_tab = (self.weight.data_ptr() + experts * wstep).to(self.device)
+        self.scales_tab = (self.scales.data_ptr() + experts * sstep).to(self.device)
 
     @classmethod
     def from_float(cls, w: torch.Tensor) -> "MXFP4ExpertBank":
@@ -236,7 +240,7 @@ def mxfp4_gather_matmul(x: torch.Tensor, w, scales: torch.Tensor | None = None, 
         raise ValueError("sorted_indices=True requires lhs_indices")
     if not isinstance(w, MXFP4ExpertBank) and scales is None:
         raise JangqError(_lib.JQ_EINVAL, "mxfp4_gather_matmul needs scales with stacked codes")
-    bank = w if isinstance(w, MXFP4ExpertBank) else MXFP4ExpertBank(w, scales)
+    bank = w if isinstance(w, MXFP4ExpertBank) else MXFP4ExpertBank(w, scales, one_call=True)
     dev = _lib.require_cuda(x, rhs_indices, lhs_indices, bank.weight)
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise JangqError(_lib.JQ_EINVAL, f"activations must be bfloat16 or float16, got {x.dtype}")

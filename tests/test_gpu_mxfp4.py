@@ -436,6 +436,26 @@ def test_captured_layer_replays_on_new_inputs(T):
 
 
 @pytest.mark.gpu
+def test_bank_tables_are_there_for_other_streams():
+    w, s = jq.mxfp4_quantize(torch.zeros((5, 8, 64), device="cuda"))
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)                        # some tens of milliseconds of the current stream
+    bank = jq.MXFP4ExpertBank(w, s)
+    with torch.cuda.stream(other):
+        codes, scales = bank.codes_tab.cpu(), bank.scales_tab.cpu()
+    assert codes.tolist() == [w.data_ptr() + e * 8 * 32 for e in range(5)]
+    assert scales.tolist() == [s.data_ptr() + e * 8 * 2 for e in range(5)]
+    graph, x, idx = torch.cuda.CUDAGraph(), torch.ones((70, 64), device="cuda", dtype=torch.bfloat16), torch.zeros((70, 1), dtype=torch.int32, device="cuda")
+    with torch.cuda.graph(graph):                        # stacked codes, and a bank, inside a capture
+        y = jq.mxfp4_gather_matmul(x, w, s, rhs_indices=idx)
+        z = jq.mxfp4_gather_matmul(x, jq.MXFP4ExpertBank(w, s), rhs_indices=idx)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, torch.zeros_like(y)) and torch.equal(z, y)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once():
     wq, s, v = _packed(3, (640, 512))
     xs = [_rand(i, (m, 512), "bf16") for i, m in enumerate((1, 12, 70, 300))]
