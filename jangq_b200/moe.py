@@ -443,10 +443,11 @@ def _moe_layer_mxfp4(x, idx, w, gate, up, down, swiglu_limit, shared, expert_bas
         if use_sorted and gate.gemm_ok and down.gemm_ok:
             sp = SortedPairs(idx32, gate.E, expert_base, tile_m=_lib.MOE_GEMM_TILE_M)
             xs = _gather_rows(x, sp, k)
+            (gate_codes, gate_scales), (up_codes, up_scales) = gate.tables(), up.tables()
             _lib.check(lib.jq_mxfp4_moe_gate_up_swiglu(
                 xs.data_ptr(), dt, sp.n, xs.stride(0), sp.offsets.data_ptr(), sp.tile_expert.data_ptr(), sp.tile_row0.data_ptr(),
-                sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, gate.codes_tab.data_ptr(), gate.scales_tab.data_ptr(),
-                up.codes_tab.data_ptr(), up.scales_tab.data_ptr(), I, gate.K, wf.data_ptr(), sp.order.data_ptr(),
+                sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, gate_codes.data_ptr(), gate_scales.data_ptr(),
+                up_codes.data_ptr(), up_scales.data_ptr(), I, gate.K, wf.data_ptr(), sp.order.data_ptr(),
                 float(swiglu_limit), h.data_ptr(), h.stride(0), st))
             y, inv = expert_gemm(h, sp, down), sp.inv.data_ptr()
         else:

@@ -147,7 +147,7 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
 
 class MXFP4ExpertBank:
     """MXFP4 weights of E experts for one projection: `weight` int32/uint32 [E, N, K/8], `scales` uint8 [E, N, K/32].
-    Device pointer tables for the grouped products are built once (one_call: for use on the stream that is current now)."""
+    The device pointer tables of the grouped products are built once (one_call: for a product that follows at once, by it)."""
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, one_call: bool = False):
         self.device = _lib.require_cuda(weight, scales)
@@ -155,16 +155,32 @@ class MXFP4ExpertBank:
             raise JangqError(_lib.JQ_EINVAL, f"stacked expert weight must be [E, N, K/8], got {tuple(weight.shape)}")
         self.weight, self.scales, self.K = _check_pair(weight, scales, "expert codes")
         self.E, self.N = self.weight.shape[:2]
-        wstep, sstep = self.N * self.K // 2, self.N * self.K // BLOCK
         if self.E < 1 or self.N < 1:
             raise JangqError(_lib.JQ_EINVAL, f"a bank holds at least one row of one expert, got {tuple(weight.shape)}")
         # The pointers are complete when the constructor returns: a product on another stream that does not wait for this one would
-        # read wrong numbers from weights on their way, but fault on pointers.  A capture (and a bank of one call, whose products
-        # follow on the same stream) cannot wait.
-        wait = not (one_call or torch.cuda.is_current_stream_capturing())
-        experts = torch.arange(self.E, dtype=torch.int64, device="cpu" if wait else self.device)
-        self.codes_tab = (self.weight.data_ptr() + experts * wstep).to(self.device)
-        self.scales_tab = (self.scales.data_ptr() + experts * sstep).to(self.device)
+        # read wrong numbers from weights on their way, but fault on pointers.  A capture cannot wait, and a table that it fills holds
+        # nothing until a replay; a bank made in one leaves the tables to the products, each of which builds its own.
+        self._tables = None
+        with _lib.on_device(self.device):
+            if not one_call and not torch.cuda.is_current_stream_capturing():
+                self._tables = tuple(t.to(self.device) for t in self._pointers("cpu"))
+
+    def _pointers(self, device):
+        """int64 tables of the experts' codes and scales."""
+        return tuple(torch.arange(p, p + self.E * step, step, dtype=torch.int64, device=device)
+                     for p, step in ((self.weight.data_ptr(), self.N * self.K // 2), (self.scales.data_ptr(), self.N * self.K // BLOCK)))
+
+    def tables(self):
+        """Device pointer tables (codes, scales) for work on the current stream; the caller holds them until it is launched."""
+        return self._tables or self._pointers(self.device)
+
+    @property
+    def codes_tab(self) -> torch.Tensor:
+        return self.tables()[0]
+
+    @property
+    def scales_tab(self) -> torch.Tensor:
+        return self.tables()[1]
 
     @classmethod
     def from_float(cls, w: torch.Tensor) -> "MXFP4ExpertBank":
@@ -218,11 +234,12 @@ def expert_gemm(x_sorted: torch.Tensor, sp, bank: MXFP4ExpertBank, scatter: bool
     """The grouped product over expert-sorted rows (moe.SortedPairs); scatter=True stores the rows where their pairs stand,
     and zeros for the pairs of no expert of the bank."""
     lib = _lib.load()
+    codes, scales = bank.tables()
     y = x_sorted.new_empty((x_sorted.shape[0], bank.N))
     _lib.check(lib.jq_mxfp4_moe_gemm(x_sorted.data_ptr(), _lib.dtype_id(x_sorted.dtype), sp.n, x_sorted.stride(0),
                                      sp.offsets.data_ptr(), sp.tile_expert.data_ptr(), sp.tile_row0.data_ptr(),
-                                     sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, bank.codes_tab.data_ptr(),
-                                     bank.scales_tab.data_ptr(), bank.N, bank.K, sp.order.data_ptr() if scatter else None,
+                                     sp.num_tiles.data_ptr(), sp.max_tiles, sp.tile_m, codes.data_ptr(),
+                                     scales.data_ptr(), bank.N, bank.K, sp.order.data_ptr() if scatter else None,
                                      sp.inv.data_ptr() if scatter else None, y.data_ptr(), bank.N,
                                      _lib.stream_ptr(x_sorted.device)))
     return y
