@@ -5,8 +5,10 @@
 // rate, and eight codes put together by permutes or shifts take 28 cycles of a scheduler, eight cycles with the conversion
 // instruction to f16 pairs.  So the operands of the warp MMAs (m16n8k16, the weights as the 16-row operand) are f16: the codes'
 // plain values, and activations scaled per block of 32 by a power of two (none for f16 activations, which are exact; a
-// bf16 one is exact unless it is below 2^-29 of the largest of its block, and off by 2^-40 of that at most).  Each block's
-// sums, 32 products, leave the MMA in f32 and are multiplied by the two powers of two on their way into the row's sum.
+// bf16 one is exact unless it is below 2^-29 of the largest of its block, and off by 2^-39 of that at most).  Each block's
+// sums, 32 products, leave the MMA in f32 and are multiplied by the two powers of two on their way into the row's sum, the
+// activations' first: it is held 2^10 smaller and the weight's 2^10 larger, so that the first product, up to 2^136 for the largest
+// activations, stays finite; it is exact at the lower end too, a multiple of 2^-144.
 //   up to 2 rows   the MMA's eight columns are four blocks of two tokens: a lane reads one whole block, its activations stand
 //                  in that block's column alone, and one multiplication per two columns and row puts in the scales
 //   up to 8 rows   the columns are tokens, block after block; more rows take further launches
@@ -50,6 +52,7 @@ constexpr int MXV_RING = MXV_WARPS * MXV_STAGES * MXV_STAGE;
 constexpr int MXV_MAX_SMEM = 226 * 1024;
 constexpr int MXV_EXTRA = 128;                                          // a row of zeros, and what tokens past the last read
 constexpr int MXV_PAD = 32;                                             // halves between activation rows, past whole stretches
+constexpr int MXV_SHIFT = 10;                                           // powers of two between the activations' scales and the weights'
 
 // COLS: one or two tokens (the columns are blocks); else up to eight
 template <bool COLS> __host__ __device__ constexpr int mxv_tokens() { return COLS ? 2 : 8; }
@@ -74,17 +77,25 @@ template <int I> __device__ __forceinline__ float mx_scale_any(uint32_t w) {
     const uint32_t f = __float_as_uint(mx_scale<I>(w));
     return __uint_as_float(f == 0u ? 0x00400000u : (f == 0x7F800000u ? 0x7FC00000u : f));
 }
-// the four of a word; fast: none of the warp's bytes is 0 or 255
-__device__ __forceinline__ void mx_scales4(uint32_t w, bool fast, float (&f)[4]) {
+// The four of a word, times 2^SHIFT where fast.  fast: none of the warp's bytes leaves the normal numbers then (0 and 255 without a
+// shift; with one a zero byte is in range, and those from 255 - SHIFT on are not).
+template <int SHIFT> __device__ __forceinline__ void mx_scales4(uint32_t w, bool fast, float (&f)[4]) {
     if (fast) {
+        w += SHIFT * 0x01010101u;
         f[0] = mx_scale<0>(w); f[1] = mx_scale<1>(w); f[2] = mx_scale<2>(w); f[3] = mx_scale<3>(w);
     } else {
         f[0] = mx_scale_any<0>(w); f[1] = mx_scale_any<1>(w); f[2] = mx_scale_any<2>(w); f[3] = mx_scale_any<3>(w);
     }
 }
+// bit 7 of every byte that is out of the fast form's range
+template <int SHIFT> __device__ __forceinline__ uint32_t mx_slow_bytes(uint32_t w) {
+    const uint32_t low = w & 0x7F7F7F7Fu, high = (low + (SHIFT + 1) * 0x01010101u) & w;
+    return (SHIFT > 0 ? high : high | ~((low + 0x7F7F7F7Fu) | w)) & 0x80808080u;
+}
 // One activation row into shared memory as f16, zeros from K to the end of its last stretch.  bf16: block b is multiplied by
-// 2^-e and scales[b * stride] = 2^e, e such that the block's largest is in [2^14, 2^15) (not below 2^-100: smaller blocks lose
-// bits below 2^-125).  A block with an infinity or a NaN keeps those as they are and nothing else: the products are the same.
+// 2^-e and scales[b * stride] = 2^(e - MXV_SHIFT), e such that the block's largest is in [2^14, 2^15), but not below -109: from
+// there on every bf16 number, a multiple of 2^-133, is one of f16's smallest step.  A block with an infinity or a NaN keeps those as
+// they are and nothing else: the products are the same.
 // Threads 4i .. 4i + 3 share a block.
 template <typename AT>
 __device__ __forceinline__ void stage_row(const uint16_t* __restrict__ src, int nblk, int nunit, uint16_t* dst, float* scales, int stride,
@@ -100,7 +111,7 @@ __device__ __forceinline__ void stage_row(const uint16_t* __restrict__ src, int 
             const uint32_t four = 0xFu << (threadIdx.x & 28);
             m = max(m, __shfl_xor_sync(four, m, 1));
             m = max(m, __shfl_xor_sync(four, m, 2));
-            const int ex = (int)(m >> 7), e = ex == 255 ? 0 : max(ex - 141, -100);
+            const int ex = (int)(m >> 7), e = ex == 255 ? 0 : max(ex - 141, -109);
             const float mult = __uint_as_float((uint32_t)(127 - e) << 23);
             uint32_t o[4];
 #pragma unroll
@@ -113,7 +124,7 @@ __device__ __forceinline__ void stage_row(const uint16_t* __restrict__ src, int 
                 o[i] = Act<__half>::pack_hi(lo * mult, hi * mult);
             }
             v = make_uint4(o[0], o[1], o[2], o[3]);
-            if ((c & 3) == 0) scales[(c >> 2) * stride] = __uint_as_float((uint32_t)(127 + e) << 23);
+            if ((c & 3) == 0) scales[(c >> 2) * stride] = __uint_as_float((uint32_t)(127 - MXV_SHIFT + e) << 23);
         }
         *reinterpret_cast<uint4*>(dst + c * 8) = v;
     }
@@ -172,7 +183,7 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
     using H = Act<__half>;
     extern __shared__ __align__(16) uint8_t mxv_smem[];
     constexpr bool SCALED = umma_fmt<AT>() == 1u;
-    constexpr int TOK = mxv_tokens<COLS>();
+    constexpr int TOK = mxv_tokens<COLS>(), SHIFT = SCALED ? MXV_SHIFT : 0;
     overlap_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int KS = 1 << a.ks_log2, ks = warp & (KS - 1), rg = warp >> a.ks_log2, rows = 16 * (MXV_WARPS >> a.ks_log2);
@@ -296,9 +307,10 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                         p1[i] = (p1[i] & keep) | (0x7F7F7F7Fu & ~keep);
                     }
                 }
-                // a byte of 0 or 255 among them: the four lanes of a row pair look at a word each
-                const uint32_t mine = t & 2 ? (t & 1 ? p1[1] : p1[0]) : (t & 1 ? p0[1] : p0[0]), low = mine & 0x7F7F7F7Fu;
-                const bool fast = !__any_sync(0xFFFFFFFFu, (((low + 0x01010101u) & mine) | ~((low + 0x7F7F7F7Fu) | mine)) & 0x80808080u);
+                // a byte among them that needs the other form, whose sums are 2^SHIFT smaller: the four lanes of a row pair look
+                // at a word each
+                const uint32_t mine = t & 2 ? (t & 1 ? p1[1] : p1[0]) : (t & 1 ? p0[1] : p0[0]);
+                const bool fast = !__any_sync(0xFFFFFFFFu, mx_slow_bytes<SHIFT>(mine));
                 float* out = part + (ti * MXV_WARPS + warp) * (TOK * 17);
                 if constexpr (COLS) {
                     float d[2][4], v0 = 0.f, v1 = 0.f;
@@ -326,10 +338,11 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                             d[h][0] *= xe[h].x; d[h][1] *= xe[h].y; d[h][2] *= xe[h].x; d[h][3] *= xe[h].y;
                         }
                         float f[4];                        // rows g and g + 8 of the two blocks
-                        mx_scales4(prmt(p0[h], p1[h], pick), fast, f);
+                        mx_scales4<SHIFT>(prmt(p0[h], p1[h], pick), fast, f);
                         v0 = fmaf(d[h][1], f[1], fmaf(d[h][0], f[0], v0));
                         v1 = fmaf(d[h][3], f[3], fmaf(d[h][2], f[2], v1));
                     }
+                    if (SCALED && !fast) { v0 *= (float)(1 << SHIFT); v1 *= (float)(1 << SHIFT); }
                     // the two column pairs of a token
                     v0 += __shfl_xor_sync(0xFFFFFFFFu, v0, 1);
                     v1 += __shfl_xor_sync(0xFFFFFFFFu, v1, 1);
@@ -343,9 +356,9 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float f[4];
-                        mx_scales4(p0[i], fast, f);
+                        mx_scales4<SHIFT>(p0[i], fast, f);
                         f0[4 * i] = f[0]; f0[4 * i + 1] = f[1]; f0[4 * i + 2] = f[2]; f0[4 * i + 3] = f[3];
-                        mx_scales4(p1[i], fast, f);
+                        mx_scales4<SHIFT>(p1[i], fast, f);
                         f1[4 * i] = f[0]; f1[4 * i + 1] = f[1]; f1[4 * i + 2] = f[2]; f1[4 * i + 3] = f[3];
                     }
 #pragma unroll
@@ -365,6 +378,7 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                         acc[2] = fmaf(d[2], f1[b], acc[2]);
                         acc[3] = fmaf(d[3], f1[b], acc[3]);
                     }
+                    if (SCALED && !fast) { acc[0] *= (float)(1 << SHIFT); acc[1] *= (float)(1 << SHIFT); acc[2] *= (float)(1 << SHIFT); acc[3] *= (float)(1 << SHIFT); }
                     // rows g, g + 8 of tokens 2t, 2t + 1
                     float* o = out + 2 * t * 17 + g;
                     o[0] = u == ks ? acc[0] : o[0] + acc[0];
