@@ -27,6 +27,7 @@ QGEMV_MAX_M = 16
 QGEMV_MAX_BATCH = 8
 MXFP4_GEMV_MAX_K = 36864
 MOE_TILE_M = 128
+MOE_SORT_MAX_EXPERTS = 1550   # jq_moe_sort
 MOE_GEMM_TILE_M = 192   # rows per tile of the grouped GEMMs (jq_moe_gemm_tiled, jq_moe_gate_up_swiglu)
 
 _DTYPE_ID = {torch.float32: JQ_F32, torch.float16: JQ_F16, torch.bfloat16: JQ_BF16}

@@ -31,6 +31,8 @@ static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
 
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
+constexpr int SORT_SMEM = 200 * 1024;
+constexpr int SORT_MAX_EXPERTS = SORT_SMEM / ((SORT_WARPS + 1) * 4) - 1;        // one row of counters per warp, and one of starts
 
 // Stable counting sort of n = T*k expert ids, one CTA.
 //   order[p]  = flat pair index (t*k + j) of the p-th pair in expert order (ties: ascending index)
@@ -969,24 +971,24 @@ int jq_moe_sort(const int32_t* topk_idx, int64_t n_pairs, int num_experts, int e
                 int32_t* num_tiles, jq_stream_t stream) {
     using namespace jq;
     JQ_REQUIRE(n_pairs >= 0 && n_pairs < (1ll << 30), JQ_EINVAL, "bad pair count %lld", (long long)n_pairs);
-    JQ_REQUIRE(num_experts > 0 && num_experts <= 4096, JQ_EUNSUPPORTED, "num_experts must be in 1..4096");
+    JQ_REQUIRE(num_experts > 0 && num_experts <= SORT_MAX_EXPERTS, JQ_EUNSUPPORTED, "num_experts must be in 1..%d, got %d",
+               SORT_MAX_EXPERTS, num_experts);
     JQ_REQUIRE(tile_m > 0, JQ_EINVAL, "tile_m must be positive");
     JQ_REQUIRE(order && inv && expert_offsets && tile_expert && tile_row0 && num_tiles, JQ_EINVAL, "null pointer");
     JQ_REQUIRE(n_pairs == 0 || topk_idx, JQ_EINVAL, "null pointer");
     const size_t smem = (size_t)(SORT_WARPS + 1) * (num_experts + 1) * sizeof(int32_t);
-    JQ_REQUIRE(smem <= 200 * 1024, JQ_EUNSUPPORTED, "too many experts for the single-CTA sort");
     static bool attr_done[64] = {};
     int dev = 0;
     JQ_CUDA_OK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        JQ_CUDA_OK(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        JQ_CUDA_OK(cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM));
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
     if (n_pairs >= 2 * SORT_THREADS && num_experts + 1 <= SORT_THREADS) {
         // several CTAs: count, scan, place
         static bool attr2_done[64] = {};
         if (dev < 0 || dev >= 64 || !attr2_done[dev]) {
-            JQ_CUDA_OK(cudaFuncSetAttribute(moe_sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+            JQ_CUDA_OK(cudaFuncSetAttribute(moe_sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM));
             if (dev >= 0 && dev < 64) attr2_done[dev] = true;
         }
         const int chunks = (int)(n_pairs / SORT_THREADS);

@@ -195,7 +195,7 @@ class MXFP4ExpertBank:
     def use_gemm(self, pairs: int) -> bool:
         """The grouped product, not a mat-vec per pair: many pairs, or rows too long for the mat-vec (and no more experts
         than the sort in front of it takes)."""
-        return self.gemm_ok and self.E <= 4096 and (pairs >= SORT_THRESHOLD or self.K > _lib.MXFP4_GEMV_MAX_K)
+        return self.gemm_ok and self.E <= _lib.MOE_SORT_MAX_EXPERTS and (pairs >= SORT_THRESHOLD or self.K > _lib.MXFP4_GEMV_MAX_K)
 
 
 def _check_integers(idx: torch.Tensor, what: str):

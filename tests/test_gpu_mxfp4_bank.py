@@ -45,3 +45,43 @@ def test_bank_made_in_a_capture_before_and_after_its_replay(layer):
     assert torch.equal(before, want) and torch.equal(captured, want) and torch.equal(after, want) and torch.equal(aside, want)
     del graph
     assert torch.equal(use(bank, down), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E", [1550, 1551, 4097])
+@pytest.mark.parametrize("T", [20, 90])
+def test_banks_around_the_largest_sort(E, T):
+    """Routed pairs of banks that the sort takes and of larger ones, whose pairs go one by one at any number.  Sums of 32 .. 64
+    products of which each is a small multiple of 2^-4 are exact in float32; one rounding to bf16 follows."""
+    N, K, k = 32, 64, 2
+    rng = np.random.default_rng(E + T)
+    words, byte = mo.pack(rng.integers(0, 16, (E, N, K)).astype(np.uint8)), np.full((E, N, K // 32), 126, np.uint8)
+    w = mo.values(words, byte)
+    bank = jq.MXFP4ExpertBank(torch.from_numpy(words.view(np.int32)).cuda(), torch.from_numpy(byte).cuda())
+    x = torch.from_numpy(rng.integers(-4, 5, (T, K)) / 4.0).to(torch.bfloat16).cuda()
+    idx = rng.integers(0, E, (T, k))
+    idx[0], idx[1] = (0, E - 1), (E - 1, min(E - 1, 1550))
+    ids = torch.from_numpy(idx).int().cuda()
+    want = np.einsum("tk,tjnk->tjn", x.double().cpu().numpy(), w[idx])
+    y = jq.mxfp4_gather_matmul(x, bank, rhs_indices=ids).reshape(T, k, N)
+    assert torch.equal(y.cpu(), torch.from_numpy(want).to(torch.bfloat16))
+    # the whole layer, I = 64: half a step each for g, u, h, the expert's row and (few pairs) the product of the first three, with
+    # |silu'| <= 1.1 for what g does to h, and float32 sums far below
+    down = jq.MXFP4ExpertBank.from_float(_rand(5, (E, 24, K), 0.1))
+    gate = jq.MXFP4ExpertBank(bank.weight.repeat(1, 2, 1), bank.scales.repeat(1, 2, 1))
+    out = jq.moe_layer(x, ids, torch.full((T, k), 0.5, device="cuda"), gate, gate, down, out_f32=True).double().cpu().numpy()
+    d = mo.values(down.weight.cpu().numpy().view(np.uint32), down.scales.cpu().numpy())[idx]
+    g = np.concatenate([want, want], -1)
+    silu = g / (1.0 + np.exp(-g))
+    h = 0.5 * silu * g
+    spread = 2 * np.abs(h) + 0.5 * (1.1 * np.abs(g) + np.abs(silu)) * np.abs(g)
+    ref, mag = np.einsum("tjk,tjnk->tn", h, d), np.einsum("tjk,tjnk->tn", spread + np.abs(h), np.abs(d))
+    assert np.all(np.abs(out - ref) <= (2.0 ** -8 + 2.0 ** -14) * mag)
+
+
+def test_largest_sort_is_the_library_s():
+    lib, L = jq._lib.load(), jq._lib
+    p, most = 1024, L.MOE_SORT_MAX_EXPERTS
+    assert lib.jq_moe_sort(p, 64, most + 1, 0, p, p, p, 192, p, p, p, None) == L.JQ_EUNSUPPORTED
+    assert lib.jq_moe_sort(p, 64, 0, 0, p, p, p, 192, p, p, p, None) == L.JQ_EUNSUPPORTED
+    assert lib.jq_moe_sort(p, 64, most, 0, p, p, p, 0, p, p, p, None) == L.JQ_EINVAL         # only the tile is wrong
