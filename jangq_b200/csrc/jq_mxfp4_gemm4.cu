@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "jq_mxfp4.cuh"
+#include "jq_mxfp4_form.cuh"
 
 namespace jq {
 
@@ -636,13 +637,6 @@ mxfp4_gemm4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(G4_NCOLS) : "memory");
 }
 
-// What the choice of a form goes by (us on B200; K stages of 256 codes).  One CTA per tile: 2 once, then per wave of tiles 2.2 and
-// 0.205 + 0.00085 tn per stage; a split of K adds 0.7 + 0.011 tn.  CTA pairs: 7.2 once, then 0.04 + 0.0015 tn per stage and round.
-// Measured: 16 rows 4096x4096 7.6 unsplit, 6.5 by 2, 6.0 by 4, 10.2 in pairs; 128 rows 2048x8192 12.7, 11.0, 9.0, 15.4; 256 rows
-// 4096x4096 9.0, 9.0, 15.4, 12.3; 1024 rows 4096x4096 16.0, 30.6, 53.5, 14.3; 4096 rows 14336x4096 181 unsplit, 96 to 98 in pairs.
-constexpr double G4_T_ONCE = 2.0, G4_T_WAVE = 2.2, G4_T_STAGE = 0.205, G4_T_ROW = 0.00085, G4_T_SPLIT = 0.7, G4_T_SPLIT_ROW = 0.011;
-constexpr double G4_T_PAIR = 7.2, G4_T_PSTAGE = 0.04, G4_T_PROW = 0.0015;
-
 static int encode_codes(CUtensorMap* map, const void* codes, int64_t rows, int64_t K, int box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();
     JQ_REQUIRE(enc != nullptr, JQ_ECUDA, "cuTensorMapEncodeTiled is not available from this driver");
@@ -712,32 +706,10 @@ extern "C" int jq_mxfp4_gemm4(const uint32_t* xcodes, const uint8_t* xscales, in
     a.wscales = wscales; a.xscales = xscales; a.y = y;
     a.M = M; a.N = N; a.ldy = ldy;
     a.nblk = (int)(K / MX_BLOCK);
-    // The form with the shortest estimated time (us).
-    const int64_t sms = sm_count(), nst = (a.nblk + 7) / 8;
-    int ks = 0;
-    double best = 1e30;
-    {
-        const int64_t mt = (M + 127) / 128, tn = ((M + mt - 1) / mt + 15) / 16 * 16, tiles = (M + tn - 1) / tn * ((N + 127) / 128);
-        for (int k : {1, 2, 4}) {
-            if ((M + tn - 1) / tn >= 65536 || (k > 1 && nst < 4 * k)) continue;
-            const int64_t slots = k == 4 ? sms / 37 * 8 : sms / k, waves = (tiles + slots - 1) / slots;      // a cluster stays within a GPC
-            const double t = G4_T_ONCE + waves * (G4_T_WAVE + (double)((nst + k - 1) / k) * (G4_T_STAGE + G4_T_ROW * tn) +
-                                                  (k > 1 ? G4_T_SPLIT + G4_T_SPLIT_ROW * tn : 0.0));
-            if (t < best) { best = t; ks = k; a.tn = (int)tn; }
-        }
-    }
-    int64_t pair_tiles = 0;
-    {
-        const int64_t least = (M + G4P_TN - 1) / G4P_TN, ncol = (N + 255) / 256;
-        for (int64_t nt = least; nt <= least + 3; ++nt) {
-            const int64_t tn = ((M + nt - 1) / nt + 15) / 16 * 16, mt = (M + tn - 1) / tn, tiles = mt * ncol;
-            const double t = G4_T_PAIR + (double)((tiles + sms / 2 - 1) / (sms / 2)) * nst * (G4_T_PSTAGE + G4_T_PROW * tn);
-            if (t < best) { best = t; ks = 0; a.tn = (int)tn; a.mt = (int)mt; pair_tiles = tiles; }
-        }
-    }
-    const bool pair = ks == 0;
-    JQ_REQUIRE(!pair || pair_tiles < (1ll << 30), JQ_EUNSUPPORTED, "too many tiles for one launch (%lld)", (long long)pair_tiles);
-    a.tiles = (int)pair_tiles;
+    const Gemm4Form f = gemm4_form(M, N, a.nblk, sm_count());
+    const bool pair = f.ks == 0;
+    JQ_REQUIRE(!pair || f.tiles < (1ll << 30), JQ_EUNSUPPORTED, "too many tiles for one launch (%lld)", (long long)f.tiles);
+    a.tn = f.tn; a.mt = (int)f.mt; a.tiles = (int)f.tiles;
     a.vec = a.nblk % 16 == 0 && aligned(wscales, 16) && aligned(xscales, 16);
     a.y_pair_ok = (aligned(y, 4) && ldy % 2 == 0) ? 1 : 0;
     a.y_vec_ok = (aligned(y, 16) && ldy % 8 == 0) ? 1 : 0;
@@ -749,9 +721,9 @@ extern "C" int jq_mxfp4_gemm4(const uint32_t* xcodes, const uint8_t* xscales, in
     rc = encode_codes(&xmap, xcodes, M, K, pair ? a.tn / 2 : a.tn);
     if (rc != JQ_OK) return rc;
     JQ_DISPATCH_DTYPE(y_dtype, OT,
-        if (ks == 1) return launch_gemm4<OT, 1>(wmap, xmap, a, (cudaStream_t)stream);
-        if (ks == 2) return launch_gemm4<OT, 2>(wmap, xmap, a, (cudaStream_t)stream);
-        if (ks == 4) return launch_gemm4<OT, 4>(wmap, xmap, a, (cudaStream_t)stream);
+        if (f.ks == 1) return launch_gemm4<OT, 1>(wmap, xmap, a, (cudaStream_t)stream);
+        if (f.ks == 2) return launch_gemm4<OT, 2>(wmap, xmap, a, (cudaStream_t)stream);
+        if (f.ks == 4) return launch_gemm4<OT, 4>(wmap, xmap, a, (cudaStream_t)stream);
         return launch_gemm4<OT, 0>(wmap, xmap, a, (cudaStream_t)stream))
     return JQ_OK;
 }
