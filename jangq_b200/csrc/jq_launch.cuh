@@ -6,17 +6,17 @@
 namespace jq {
 
 // First statement of such a kernel, in every thread: the successor may be scheduled from here on, and no memory is touched
-// before all earlier work of the stream is complete and visible.
+// before all earlier work of the stream is complete and visible.  No effect in a launch without the attribute.
 __device__ __forceinline__ void overlap_enter() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 template <typename... KArgs, typename... Args>
-static cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, Args... args) {
+static cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -24,7 +24,7 @@ static cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, unsign
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
 }  // namespace jq

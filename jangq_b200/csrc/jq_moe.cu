@@ -2,33 +2,13 @@
 // row gather, SwiGLU with routing weight, and the top-k combine.  The matmuls themselves are the
 // grouped mode of the tensor-core GEMM (jq_qgemm.cu) and the gather mode of the mat-vec
 // (jq_qgemv.cu).  All of these are small, bandwidth-bound index/elementwise kernels.
+#include "jq_launch.cuh"
 #include "jq_mma.cuh"
 
 namespace jq {
 
-// The small kernels of the few-token path are launched with programmatic stream serialization: their CTAs
-// may be scheduled while the predecessor still runs, and they touch memory only after griddepcontrol.wait
-// (which returns once the predecessor has completed and flushed), so the launch latency of a chain of
-// tiny dependent kernels overlaps.  The instruction is a no-op for a launch without the attribute.
-__device__ __forceinline__ void pdl_enter() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-
+// The small kernels of the few-token path are launched over the end of their predecessor (jq_launch.cuh), so the launch latency of a
+// chain of tiny dependent kernels overlaps.
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_SMEM = 200 * 1024;
@@ -327,7 +307,7 @@ __global__ void swiglu_kernel(const AT* __restrict__ g, const AT* __restrict__ u
                               const float* __restrict__ w, const int32_t* __restrict__ order,
                               const int32_t* __restrict__ count, AT* __restrict__ h, int64_t ld_out, int cols, int max_rows,
                               float lim) {
-    pdl_enter();
+    overlap_enter();
     const int n = count ? min(*count, max_rows) : max_rows;
     // rows of whole 16-byte vectors (the grouped-GEMM outputs): 8 elements per thread and step, same arithmetic
     const bool vec = (cols % 8 == 0) && (ld_in % 8 == 0) && (ld_out % 8 == 0) &&
@@ -459,7 +439,7 @@ route_kernel(const AT* __restrict__ x, int64_t ldx, const AT* __restrict__ wr, i
     __shared__ int is_last;
     __shared__ __align__(16) AT xn[FUSED ? 4096 : 8];
     __shared__ float part[8];
-    pdl_enter();
+    overlap_enter();
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int e = blockIdx.y * 8 + warp;
     uint4 wpre[FUSED ? 16 : 1];                            // FUSED: the expert's router row, requested before the norm
@@ -808,7 +788,7 @@ __global__ void __launch_bounds__(1024)
 residual_rmsnorm_kernel(const AT* __restrict__ x, const AT* __restrict__ y, const float* __restrict__ y_f32, int k, int H,
                         float eps, AT* __restrict__ out) {
     __shared__ float part[32];
-    pdl_enter();
+    overlap_enter();
     const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int PER = 4;                               // columns per thread held in registers (H <= 4096)
     float v[PER];
@@ -860,7 +840,7 @@ int jq_moe_route(const void* x, int act_dtype, int64_t ldx, int64_t T, int64_t H
     JQ_REQUIRE(T <= 65535, JQ_EUNSUPPORTED, "jq_moe_route is the few-token path");
     const dim3 grid((unsigned)T, (unsigned)((num_experts + 7) / 8));
     JQ_DISPATCH_DTYPE16(act_dtype, AT,
-        JQ_CUDA_OK(launch_pdl(route_kernel<AT, false>, grid, dim3(256), 0, (cudaStream_t)stream, (const AT*)x, ldx,
+        JQ_CUDA_OK(launch_overlapped(route_kernel<AT, false>, grid, dim3(256), 0, (cudaStream_t)stream, (const AT*)x, ldx,
                               (const AT*)router_w, (int)H, num_experts, k, renorm, scale, idx_out, w_out, logits_ws,
                               (int*)counters, (const AT*)nullptr, 0.f, (AT*)nullptr)))
     return JQ_OK;
@@ -909,7 +889,7 @@ int jq_moe_route_norm(const void* x, const void* res, int act_dtype, int64_t T, 
     }
     const dim3 grid((unsigned)T, (unsigned)((num_experts + 7) / 8));
     JQ_DISPATCH_DTYPE16(act_dtype, AT,
-        JQ_CUDA_OK(launch_pdl(route_kernel<AT, true>, grid, dim3(256), 0, (cudaStream_t)stream, (const AT*)x, H,
+        JQ_CUDA_OK(launch_overlapped(route_kernel<AT, true>, grid, dim3(256), 0, (cudaStream_t)stream, (const AT*)x, H,
                               (const AT*)router_w, (int)H, num_experts, k, renorm, scale, idx_out, w_out, logits_ws,
                               (int*)counters, (const AT*)res, eps, (AT*)x_out)))
     return JQ_OK;
@@ -955,7 +935,7 @@ int jq_residual_rmsnorm(const void* x, const void* y, const float* y_f32, int k,
     JQ_REQUIRE(k >= 1 && (y_f32 == nullptr || k == 1), JQ_EINVAL, "k >= 1; an f32 addend is a single row");
     JQ_REQUIRE(T <= 65535, JQ_EUNSUPPORTED, "at most 65535 rows");
     JQ_DISPATCH_DTYPE16(act_dtype, AT,
-        JQ_CUDA_OK(launch_pdl(residual_rmsnorm_kernel<AT>, dim3((unsigned)T), dim3(1024), 0, (cudaStream_t)stream,
+        JQ_CUDA_OK(launch_overlapped(residual_rmsnorm_kernel<AT>, dim3((unsigned)T), dim3(1024), 0, (cudaStream_t)stream,
                               (const AT*)x, (const AT*)y, y_f32, k, (int)H, eps, (AT*)out)))
     return JQ_OK;
 }
@@ -1031,7 +1011,7 @@ int jq_moe_swiglu(const void* gate, const void* up, int64_t ld_in, const float* 
     JQ_REQUIRE(gate && up && h, JQ_EINVAL, "null pointer");
     const int blocks = (int)(max_rows < 8 * 148 ? max_rows : 8 * 148);
     JQ_DISPATCH_DTYPE16(dtype, T,
-        JQ_CUDA_OK(launch_pdl(swiglu_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)gate,
+        JQ_CUDA_OK(launch_overlapped(swiglu_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)gate,
                               (const T*)up, ld_in, weights, order, count, (T*)h, ld_out, (int)cols, (int)max_rows, limit)))
     return JQ_OK;
 }
