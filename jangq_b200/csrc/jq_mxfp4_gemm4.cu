@@ -367,7 +367,9 @@ __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// for a thread that only read tensor memory: there is no write to release, and the releasing form takes a microsecond
+// For warps that only read tensor memory.  Their reads are over (tcgen05.wait::ld), fence::before_thread_sync and the __syncwarp
+// put them before lane 0's arrive, and the issuer's fence::after_thread_sync puts the MMAs behind its wait; no write of these
+// warps is read there, so nothing is to be released (the releasing form takes a microsecond).
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }

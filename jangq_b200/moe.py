@@ -484,7 +484,8 @@ def moe_layer(x: torch.Tensor, idx: torch.Tensor, w: torch.Tensor, gate: ExpertB
     pairs name experts of other ranks (up to 128 pairs then stay on the integer gather).  few_token_path forces
     (True) or forbids (False) the unsorted gather mat-vec path; default: below 64 pairs, as the reference.
     Banks of MXFP4 experts (MXFP4ExpertBank) are taken as well, all three or none; static_weights and few_local have no
-    meaning there, and return_slots is not provided.
+    meaning there, and return_slots is not provided.  An odd number of blocks of 32 in a row, or more experts than the sort
+    takes (1550), leave every number of tokens on the mat-vecs.
     """
     if any(isinstance(b, MXFP4ExpertBank) for b in (gate, up, down)):
         if return_slots or not all(isinstance(b, MXFP4ExpertBank) for b in (gate, up, down)):

@@ -16,7 +16,11 @@ from . import _lib
 from ._lib import JangqError
 
 BLOCK = 32
-SORT_THRESHOLD = 64      # pairs; as gather_qmm
+# Pairs from which the grouped product runs, as gather_qmm.  A mat-vec per pair takes about 4 us + pairs * (expert bytes / 4.6 TB/s),
+# the sort, the row gather and the product 12 us + 0.26 us per k-block and round of tiles, so the sizes at which they meet differ:
+# 64 pairs of 8 experts of 2048x4096 66.8 us one by one and 29.1 grouped (they meet at 24), of 32 of 1024x2048 20.5 and 29.6 (at 100), of 128
+# of 768x2048 17.3 and 37.3 (at 320), of 512 of 512x2048 13 and 31.
+SORT_THRESHOLD = 64
 # Rows that the mat-vec takes in one launch (their activations in shared memory: rows * K up to MXFP4_GEMV_MAX_K).  Beyond,
 # every weight is read again, and the tensor-core GEMM is faster: bf16, 8 rows of 14336x4096 16.8 us here, 20.4 there, 9 rows 29
 # and 20; 8 rows of 4096x4096 9.5 and 9.3, of 2048x2048 5.8 and 6.3, 9 rows 10 and 6.4; 2 rows of 4096x14336 15.3 and 19.0, 4 rows
@@ -138,7 +142,8 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
         if K % 64 == 0 and (M > MATVEC_ROWS or M * K > _lib.MXFP4_GEMV_MAX_K):
             _lib.check(lib.jq_mxfp4_gemm(xp, dt, M, ld, wp, sp, N, K, yp, N, st))
         else:
-            # an odd number of blocks is the mat-vec's, 16 rows at a time
+            # An odd number of blocks is the mat-vec's, 16 rows at a time: every 8 rows read the weights again (4096x2080: 64 rows 57 us,
+            # 2048 rows 1800; 4096x2112 8.9 and 34).
             for m0 in range(0, M, _lib.QGEMV_MAX_M):
                 _lib.check(lib.jq_mxfp4_gemv(xp + 2 * m0 * ld, dt, min(_lib.QGEMV_MAX_M, M - m0), ld, wp, sp, N, K,
                                              yp + 2 * m0 * N, N, st))
