@@ -146,29 +146,34 @@ __device__ __forceinline__ uint32_t kept_groups(const RouteArgs& a, const V* row
     return __ballot_sync(0xFFFFFFFFu, g < a.groups && rank < a.kept);
 }
 
+template <typename LT> __device__ __forceinline__ double exact_score(const RouteArgs& a, int64_t t, int e, float mx, double sum) {
+    const float lv = load_logit<LT>(a, t, e);
+    return a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
+}
 // Results of up to 32 selections from j0 on: lane j holds expert `mine`.  Returns the sum of their scores.
 template <typename LT>
 __device__ __forceinline__ double store_chosen(const RouteArgs& a, int64_t t, int lane, int j0, int n, int mine, float mx, double sum) {
     double s = 0.0, chosen;
     if (lane < n) {
-        const float lv = load_logit<LT>(a, t, mine);
-        s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
+        s = exact_score<LT>(a, t, mine, mx, sum);
         a.idx[t * a.k + j0 + lane] = mine;
     }
     chosen = s;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) chosen += __shfl_xor_sync(0xFFFFFFFFu, chosen, d);
-    if (a.k <= 32) s *= a.renorm ? (double)a.scale / (chosen + 1e-20) : (double)a.scale;
-    if (lane < n) a.w[t * a.k + j0 + lane] = (float)s;     // of more than 32: scaled when the sum is known
+    if (a.k <= 32) {                                       // of more: when the sum of all is known
+        s *= a.renorm ? (double)a.scale / (chosen + 1e-20) : (double)a.scale;
+        if (lane < n) a.w[t * a.k + j0 + lane] = (float)s;
+    }
     return chosen;
 }
-__device__ __forceinline__ void scale_chosen(const RouteArgs& a, int64_t t, int lane, double chosen) {
+template <typename LT>
+__device__ __forceinline__ void store_weights(const RouteArgs& a, int64_t t, int lane, float mx, double sum, double chosen) {
     if (a.k <= 32) return;
     const double norm = a.renorm ? (double)a.scale / (chosen + 1e-20) : (double)a.scale;
-    for (int j = lane; j < a.k; j += 32) {                 // the lane's own stores
-        float* p = a.w + t * a.k + j;
-        *p = (float)((double)*p * norm);
-    }
+#pragma unroll 1
+    for (int j = lane; j < a.k; j += 32)                   // the lane's own choices
+        a.w[t * a.k + j] = (float)(exact_score<LT>(a, t, a.idx[t * a.k + j], mx, sum) * norm);
 }
 
 // Sum of the softmax, and the choice scores of a whole token, in float64; four exponentials at a time (a row of them unrolled is
@@ -184,8 +189,7 @@ __device__ __noinline__ double exact_sum(const RouteArgs& a, int64_t t, int lane
 }
 template <typename LT>
 __device__ __forceinline__ double exact_choice(const RouteArgs& a, int64_t t, int e, float mx, double sum) {
-    const float lv = load_logit<LT>(a, t, e);
-    double c = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
+    double c = exact_score<LT>(a, t, e, mx, sum);
     if (a.bias) c += (double)a.bias[e];
     return c != c ? -(double)INFINITY : c;
 }
@@ -260,7 +264,7 @@ __device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int l
     uint32_t best, before = 0;
     int bi;                                                // register index of the lane's best
     lane_best<PER>(key, best, bi);
-    double chosen = 0.0;
+    double chosen = 0.0, used = 1.0;                       // sums of the chosen scores, and of the softmax in them
     for (int j0 = 0; j0 < a.k; j0 += 32) {
         int n = min(32, a.k - j0), mine = 0;
         bool open = false;
@@ -310,14 +314,15 @@ __device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int l
         double got;
         for (;;) {
             if (rough && !a.renorm) { sum64 = exact_sum<LT>(a, t, lane, mx); rough = false; }
-            got = store_chosen<LT>(a, t, lane, j0, n, mine, mx, sum64 != 0.0 ? sum64 : (double)sum);
+            used = sum64 != 0.0 ? sum64 : (double)sum;
+            got = store_chosen<LT>(a, t, lane, j0, n, mine, mx, used);
             if (MODE == ROUTE_LOGIT || !rough || got >= 1e-12) break;
             sum64 = exact_sum<LT>(a, t, lane, mx);
             rough = false;
         }
         chosen += got;
     }
-    scale_chosen(a, t, lane, chosen);
+    store_weights<LT>(a, t, lane, mx, used, chosen);
     return true;
 }
 
@@ -359,7 +364,7 @@ __device__ __noinline__ void route_token_exact(const RouteArgs& a, int64_t t, in
         }
         chosen += store_chosen<LT>(a, t, lane, j0, n, mine, mx, sum);
     }
-    scale_chosen(a, t, lane, chosen);
+    store_weights<LT>(a, t, lane, mx, sum, chosen);
 }
 
 // SCREEN: the order of the logits does not decide

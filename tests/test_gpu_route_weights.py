@@ -38,3 +38,18 @@ def test_renormalised_weights_of_experts_with_next_to_no_score():
     logits[:, :32] += torch.linspace(30.0, 60.0, T, device="cuda")[:, None]
     bias = torch.where(torch.arange(E, device="cuda") < 32, 0.0, torch.linspace(7.0, 9.0, E, device="cuda"))
     _check(logits, k, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k,groups,kept", [(33, 1, 1), (64, 4, 2), (96, 1, 1)])
+def test_many_experts_with_next_to_no_score(score, k, groups, kept):
+    """More than 32 experts: no score is rounded before the sum of all of them is known, below float32's range neither."""
+    T, E = 40, 128
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    logits = torch.randn((T, E), generator=gen, device="cuda") - torch.linspace(0.0, 120.0, T, device="cuda")[:, None]
+    logits[:, :32] += torch.linspace(0.0, 150.0, T, device="cuda")[:, None]
+    bias = torch.where(torch.arange(E, device="cuda") < 32, 0.0, torch.linspace(7.0, 9.0, E, device="cuda"))
+    for renorm in (True, False):
+        _check(logits, k, bias, score=score, groups=groups, groups_kept=kept, renorm=renorm)
+        _check(logits, k, None, score=score, groups=groups, groups_kept=kept, group_top=1, renorm=renorm)
