@@ -15,8 +15,8 @@
 // (the whole token again in float64: 22 us for 4096 x 256).  Where c grows with the logit alone (no bias, and at most the
 // best expert of a group counts) the order of the logits is the order of the scores, exactly.  A NaN logit counts as -inf, a
 // score of zero; +inf takes the limit.
-// Weights that are not renormalised hold the softmax's sum: it is taken in float64 then (61 tokens, 512 experts 8.4 us, 5.9 with a
-// float32 sum, whose ten roundings left weights up to three half steps off; 4096 tokens, 256 experts 11.7 and 8.1).
+// Weights that are not renormalised hold the softmax's sum: it is taken in float64 then (61 tokens, 512 experts 7.7 us, 5.9 with a
+// float32 sum, whose ten roundings left weights up to three half steps off; 4096 tokens, 256 experts 10.0 and 8.1).
 // Measured: one token, 128 experts, softmax 2.3 us (an empty launch is 2); 61 tokens, 512 experts, bias, 10 of them 6.8; sigmoid,
 // bias, the best 4 of 8 groups of 32, 8 experts: 592 tokens 5.5, 4096 tokens 13.8 (latency up to one token per scheduler, then issue
 // of the selections, the groups and the scores in like parts).
@@ -150,8 +150,8 @@ template <typename LT> __device__ __forceinline__ double exact_score(const Route
     const float lv = load_logit<LT>(a, t, e);
     return a.sigmoid ? 1.0 / (1.0 + exp(-(double)lv)) : exp_below(lv, mx) / sum;
 }
-// Results of up to 32 selections from j0 on: lane j holds expert `mine`.  Returns the sum of their scores.
-template <typename LT>
+// Results of up to 32 selections from j0 on: lane j holds expert `mine`.  Returns the sum of their scores.  MANY: k may be above 32.
+template <typename LT, bool MANY>
 __device__ __forceinline__ double store_chosen(const RouteArgs& a, int64_t t, int lane, int j0, int n, int mine, float mx, double sum) {
     double s = 0.0, chosen;
     if (lane < n) {
@@ -161,7 +161,7 @@ __device__ __forceinline__ double store_chosen(const RouteArgs& a, int64_t t, in
     chosen = s;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) chosen += __shfl_xor_sync(0xFFFFFFFFu, chosen, d);
-    if (a.k <= 32) {                                       // of more: when the sum of all is known
+    if (!MANY || a.k <= 32) {                              // of more: when the sum of all is known
         s *= a.renorm ? (double)a.scale / (chosen + 1e-20) : (double)a.scale;
         if (lane < n) a.w[t * a.k + j0 + lane] = (float)s;
     }
@@ -179,13 +179,16 @@ __device__ __forceinline__ void store_weights(const RouteArgs& a, int64_t t, int
 // Sum of the softmax, and the choice scores of a whole token, in float64; four exponentials at a time (a row of them unrolled is
 // so much code that fetching it takes longer than running it).
 template <typename LT>
-__device__ __noinline__ double exact_sum(const RouteArgs& a, int64_t t, int lane, float mx) {
+__device__ __forceinline__ double exact_sum_here(const RouteArgs& a, int64_t t, int lane, float mx) {
     double sum = 0.0;
 #pragma unroll 4
     for (int e = lane; e < a.E; e += 32) sum += exp_below(load_logit<LT>(a, t, e), mx);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     return sum == 0.0 ? 1.0 : sum;                         // a row of -inf: every score is zero
+}
+template <typename LT> __device__ __noinline__ double exact_sum(const RouteArgs& a, int64_t t, int lane, float mx) {
+    return exact_sum_here<LT>(a, t, lane, mx);
 }
 template <typename LT>
 __device__ __forceinline__ double exact_choice(const RouteArgs& a, int64_t t, int e, float mx, double sum) {
@@ -200,8 +203,23 @@ __device__ __noinline__ void exact_row(const RouteArgs& a, int64_t t, int lane, 
     __syncwarp();
 }
 
+// The n candidates, one per lane, in the order of their exact scores (place: n ints).
+template <typename LT>
+__device__ __noinline__ int exact_order(const RouteArgs& a, int64_t t, int lane, int n, int mine, int* place, float mx, double sum) {
+    const uint64_t key = lane < n ? order_key(exact_choice<LT>(a, t, mine, mx, sum)) : 0ull;
+    int rank = 0;
+    for (int o = 0; o < n; ++o) {
+        const uint64_t other = __shfl_sync(0xFFFFFFFFu, key, o);
+        const int oe = __shfl_sync(0xFFFFFFFFu, mine, o);
+        rank += other > key || (other == key && oe < mine) ? 1 : 0;
+    }
+    if (lane < n) place[rank] = mine;
+    __syncwarp();
+    return lane < n ? place[lane] : 0;
+}
+
 // One token on 32-bit keys (row: E doubles of shared memory, or floats where the logits decide).  Returns false (the same in
-// every lane, nothing written) where more than 32 experts are too close to tell.
+// every lane) where the token is to be done in float64: more than 32 experts too close to tell, or weights that hold the screen's sum.
 template <typename LT, int PER, RouteMode MODE>
 __device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int lane, void* row, const float (&l)[PER], float mx) {
     const int E = a.E;
@@ -264,7 +282,7 @@ __device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int l
     uint32_t best, before = 0;
     int bi;                                                // register index of the lane's best
     lane_best<PER>(key, best, bi);
-    double chosen = 0.0, used = 1.0;                       // sums of the chosen scores, and of the softmax in them
+    double chosen = 0.0;
     for (int j0 = 0; j0 < a.k; j0 += 32) {
         int n = min(32, a.k - j0), mine = 0;
         bool open = false;
@@ -292,37 +310,22 @@ __device__ __forceinline__ bool route_token(const RouteArgs& a, int64_t t, int l
                 if (j >= n) n = j + 1;
         }
         if constexpr (MODE == ROUTE_SCREEN) {
-            if (open) {                                    // k <= 32 here: order the n candidates by their exact scores
+            if (open) {                                    // k <= 32 here
                 if (!a.sigmoid && sum64 == 0.0) sum64 = exact_sum<LT>(a, t, lane, mx);
-                const uint64_t k64 = lane < n ? order_key(exact_choice<LT>(a, t, mine, mx, sum64)) : 0ull;
-                int rank = 0;
-                for (int o = 0; o < n; ++o) {
-                    const uint64_t other = __shfl_sync(0xFFFFFFFFu, k64, o);
-                    const int oe = __shfl_sync(0xFFFFFFFFu, mine, o);
-                    rank += other > k64 || (other == k64 && oe < mine) ? 1 : 0;
-                }
-                int* place = reinterpret_cast<int*>(row);  // E >= n of them
-                if (lane < n) place[rank] = mine;
-                __syncwarp();
-                mine = lane < n ? place[lane] : 0;
+                mine = exact_order<LT>(a, t, lane, n, mine, reinterpret_cast<int*>(row), mx, sum64);
             }
             n = min(32, a.k - j0);
         }
         // A renormalised weight does not hold the sum, so the screen's (or none, where the logits decide) does for it, unless the
         // chosen scores are so small, against the largest, that the 1e-20 beside their own sum counts.
-        bool rough = !a.sigmoid && sum64 == 0.0;
-        double got;
-        for (;;) {
-            if (rough && !a.renorm) { sum64 = exact_sum<LT>(a, t, lane, mx); rough = false; }
-            used = sum64 != 0.0 ? sum64 : (double)sum;
-            got = store_chosen<LT>(a, t, lane, j0, n, mine, mx, used);
-            if (MODE == ROUTE_LOGIT || !rough || got >= 1e-12) break;
-            sum64 = exact_sum<LT>(a, t, lane, mx);
-            rough = false;
-        }
-        chosen += got;
+        // (A call costs a copy of the arguments at the kernel's start, which the form without others is spared.)
+        if (!a.sigmoid && !a.renorm && sum64 == 0.0)
+            sum64 = MODE == ROUTE_LOGIT ? exact_sum_here<LT>(a, t, lane, mx) : exact_sum<LT>(a, t, lane, mx);
+        const double got = store_chosen<LT, MODE == ROUTE_LOGIT>(a, t, lane, j0, n, mine, mx, sum64 != 0.0 ? sum64 : (double)sum);
+        if constexpr (MODE == ROUTE_LOGIT) chosen += got;
+        else if (!a.sigmoid && sum64 == 0.0 && got < 1e-12) return false;
     }
-    store_weights<LT>(a, t, lane, mx, used, chosen);
+    if constexpr (MODE == ROUTE_LOGIT) store_weights<LT>(a, t, lane, mx, sum64 != 0.0 ? sum64 : 1.0, chosen);
     return true;
 }
 
@@ -362,7 +365,7 @@ __device__ __noinline__ void route_token_exact(const RouteArgs& a, int64_t t, in
             }
             __syncwarp();
         }
-        chosen += store_chosen<LT>(a, t, lane, j0, n, mine, mx, sum);
+        chosen += store_chosen<LT, true>(a, t, lane, j0, n, mine, mx, sum);
     }
     store_weights<LT>(a, t, lane, mx, sum, chosen);
 }

@@ -301,7 +301,7 @@ def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch
     # the pitch of a single row says nothing, and a broadcast one (0) names no rows
     if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
         logits = logits.contiguous()
-    if any(abs(v) >= 1 << 31 for v in (groups, groups_kept, group_top)):              # the library sees 32 bits of them
+    if not (abs(groups) < 1 << 31 and abs(groups_kept) < 1 << 31 and abs(group_top) < 1 << 31):       # the library sees 32 bits of them
         raise JangqError(_lib.JQ_EINVAL, f"groups {groups}, groups_kept {groups_kept} and group_top {group_top} must fit 32 bits")
     if not 1 <= k <= E:                  # here, before a table of that size is asked for
         raise JangqError(_lib.JQ_EINVAL, f"k must be 1 to the number of experts ({E}), got {k}")
