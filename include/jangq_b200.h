@@ -229,7 +229,8 @@ size_t jq_moe_sort_max_tiles(int64_t n_pairs, int num_experts, int tile_m);
  * [expert_base, expert_base + num_experts) (another rank's, under expert parallelism) are dropped:
  * inv = -1.  expert_offsets[num_experts + 1]; expert_offsets[num_experts] = kept pairs.  Also emits
  * the tile list of the grouped GEMM: tile t covers sorted rows tile_row0[t] .. of expert
- * tile_expert[t]; *num_tiles tiles.  All outputs are device arrays; nothing syncs. */
+ * tile_expert[t]; *num_tiles tiles.  All outputs are device arrays; nothing syncs.  num_experts <= 1550 (the counters of one
+ * CTA's warps in shared memory). */
 int jq_moe_sort(const int32_t* topk_idx, int64_t n_pairs, int num_experts, int expert_base,
                 int32_t* order, int32_t* inv, int32_t* expert_offsets, int tile_m,
                 int32_t* tile_expert, int32_t* tile_row0, int32_t* num_tiles, jq_stream_t stream);
@@ -492,7 +493,8 @@ int jq_ep_combine_residual_rmsnorm(const void* x, const void* y, int k, int64_t 
  *   groups > 1: experts [g E/groups, (g+1) E/groups) form group g, whose score is the sum of its group_top (1 or 2)
  *   largest c; experts outside the groups_kept best groups (ties: the lower group) are not chosen
  *   idx = the k largest c, descending, ties to the lower expert;   w = s[idx], / (their sum + 1e-20) when renorm, * scale
- * c is compared in float64, so the choice is the one of the exact scores up to 1e-16.  A NaN logit counts as -inf (score
+ * c is compared in float64, so the choice is the one of the exact scores up to 1e-16; w is computed in float64 and rounded
+ * once.  A NaN logit counts as -inf (score
  * zero); k may not exceed the experts of the kept groups.  With softmax, no bias and one group it is jq_moe_topk's
  * selection.  logits [T, ld >= num_experts] f32, f16 or bf16; idx_out int32 [T, k], w_out f32 [T, k]; num_experts <= 1024,
  * groups <= 32.  The reference's routers: dots3/ops.py:149-162 and dsv41/model.py:1171-1191. */

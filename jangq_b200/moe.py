@@ -285,8 +285,8 @@ def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch
     s = softmax(logits) or sigmoid(logits); experts are chosen by c = s + bias (bias [E], for the choice only).  With
     groups > 1 the E / groups experts of a group stand together, a group's score is the sum of its `group_top` (1 or 2)
     largest c, and only experts of the `groups_kept` best groups can be chosen.  idx is in descending order of c, ties to
-    the lower expert (and the lower group); w = s[idx], divided by their sum + 1e-20 with renorm, times scale.  NaN
-    logits count as -inf.  E <= 1024, groups <= 32."""
+    the lower expert (and the lower group); w = s[idx], divided by their sum + 1e-20 with renorm, times scale, in 64 bits
+    and rounded once.  NaN logits count as -inf.  E <= 1024, groups <= 32."""
     dev = _lib.require_cuda(logits, bias)
     lib = _lib.load()
     if logits.dim() != 2:
