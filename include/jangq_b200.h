@@ -494,9 +494,8 @@ int jq_ep_combine_residual_rmsnorm(const void* x, const void* y, int k, int64_t 
  *   largest c; experts outside the groups_kept best groups (ties: the lower group) are not chosen
  *   idx = the k largest c, descending, ties to the lower expert;   w = s[idx], / (their sum + 1e-20) when renorm, * scale
  * c is compared in float64, so the choice is the one of the exact scores up to 1e-16; w is computed in float64 and rounded
- * once.  A NaN logit counts as -inf (score
- * zero); k may not exceed the experts of the kept groups.  With softmax, no bias and one group it is jq_moe_topk's
- * selection.  logits [T, ld >= num_experts] f32, f16 or bf16; idx_out int32 [T, k], w_out f32 [T, k]; num_experts <= 1024,
+ * once.  A NaN logit counts as -inf (score zero); k may not exceed the experts of the kept groups.  With softmax, no bias and
+ * one group it is jq_moe_topk's selection.  logits [T, ld >= num_experts] f32, f16 or bf16; idx_out int32 [T, k], w_out f32 [T, k]; num_experts <= 1024,
  * groups <= 32.  The reference's routers: dots3/ops.py:149-162 and dsv41/model.py:1171-1191. */
 int jq_moe_route_topk(const void* logits, int logits_dtype, int64_t ld, int64_t T, int num_experts, int k, int score,
                       const float* bias, int groups, int groups_kept, int group_top, int renorm, float scale,
@@ -516,8 +515,8 @@ int jq_mxfp4_dequantize(const uint32_t* codes, const uint8_t* scales, int64_t ro
                         jq_stream_t stream);
 
 /* y[M, N] = x[M, K] . deq(w)[N, K]^T, x and y of one 16-bit type, f32 sums.  In the tensor-core forms the weight enters in
- * x's type: exact in bf16, rounded once in f16 (scales below 2^-23, and overflow to infinity above 2^13).  x 16-byte
- * aligned with ldx % 8 == 0, codes 16-byte, scales 4-byte aligned.
+ * x's type: exact in bf16 (infinite from 2^128 on), rounded once in f16 (scales below 2^-23, and overflow to infinity above
+ * 2^13).  x 16-byte aligned with ldx % 8 == 0, codes 16-byte, scales 4-byte aligned.
  *   jq_mxfp4_gemm: any M, K % 64 == 0 (tensor cores)
  *   jq_mxfp4_gemv: M <= 16, K % 32 == 0 up to 36864.  Its products are of f16 pairs in any case: bf16 activations are
  *   scaled per block of 32 by a power of two, and those below 2^-29 of the largest of their block rounded (by less than

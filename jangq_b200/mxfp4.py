@@ -91,7 +91,8 @@ def mxfp4_quantize(w: torch.Tensor):
 
 
 def mxfp4_dequantize(wq: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The numbers a packed pair stands for -> [.., K], rounded once to `dtype` (exact in bfloat16 and float32)."""
+    """The numbers a packed pair stands for -> [.., K], rounded once to `dtype` (exact in bfloat16 and float32 but for
+    2^128 and above, which mxfp4_quantize does not give)."""
     dev = _lib.require_cuda(wq, scales)
     lib = _lib.load()
     wq, scales, K = _check_pair(wq, scales)
@@ -107,8 +108,9 @@ def mxfp4_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, x_scale
     """y[.., N] = x[.., K] . deq(w, scales)[N, K]^T with float32 sums.
 
     x bfloat16 or float16: few rows run the mat-vec kernel, more the tensor-core GEMM; the output has x's type.  In
-    the GEMM the weight enters in it (exact in bfloat16; in float16 rounded once, and beyond 65504 infinite); the mat-vec
-    rounds bfloat16 activations below 2^-29 of the largest of their block of 32, by less than 2^-39 of it.
+    the GEMM the weight enters in it (exact in bfloat16, but infinite from 2^128 on; in float16 rounded once, and
+    beyond 65504 infinite); the mat-vec rounds bfloat16 activations below 2^-29 of the largest of their block of 32, by
+    less than 2^-39 of it.
     x int32 codes [.., K/8] with x_scales uint8 [.., K/32] (mxfp4_quantize of the activations): both operands go to the
     tensor cores in 4 bits; the output type is `dtype` (bfloat16 by default)."""
     dev = _lib.require_cuda(x, w, scales, x_scales)
