@@ -307,8 +307,8 @@ mxfp4_gemv_kernel(const MxGemvArgs a) {
                         p1[i] = (p1[i] & keep) | (0x7F7F7F7Fu & ~keep);
                     }
                 }
-                // a byte among them that needs the other form, whose sums are 2^SHIFT smaller: the four lanes of a row pair look
-                // at a word each
+                // a byte among them that needs the other form, whose sums are 2^SHIFT smaller (and whole multiples of 2^-139, far
+                // below the smallest numbers of the results): the four lanes of a row pair look at a word each
                 const uint32_t mine = t & 2 ? (t & 1 ? p1[1] : p1[0]) : (t & 1 ? p0[1] : p0[0]);
                 const bool fast = !__any_sync(0xFFFFFFFFu, mx_slow_bytes<SHIFT>(mine));
                 float* out = part + (ti * MXV_WARPS + warp) * (TOK * 17);
