@@ -17,9 +17,9 @@
 // score of zero; +inf takes the limit.
 // Weights that are not renormalised hold the softmax's sum: it is taken in float64 then (61 tokens, 512 experts 7.7 us, 5.9 with a
 // float32 sum, whose ten roundings left weights up to three half steps off; 4096 tokens, 256 experts 10.0 and 8.1).
-// Measured: one token, 128 experts, softmax 2.3 us (an empty launch is 2); 61 tokens, 512 experts, bias, 10 of them 6.8; sigmoid,
-// bias, the best 4 of 8 groups of 32, 8 experts: 592 tokens 5.5, 4096 tokens 13.8 (latency up to one token per scheduler, then issue
-// of the selections, the groups and the scores in like parts).
+// Measured: one token, 128 experts, softmax 2.5 us (an empty launch is 2); 61 tokens, 512 experts, bias, 10 of them 6.8; sigmoid,
+// bias, the best 4 of 8 groups of 32, 8 experts: 592 tokens 5.6, 4096 tokens 12 to 14 by how close their scores lie (latency up to one
+// token per scheduler, then issue of the selections, the groups and the scores in like parts).
 #include "jq_launch.cuh"
 
 namespace jq {
